@@ -154,7 +154,8 @@ def _quantized(x):
     """(values in 8 bits, scales [K / 128, rows]) of x [rows, K] in 32 bits."""
     b = _in_blocks(x)
     tiny = torch.finfo(torch.float32).tiny
-    s = (b.abs().amax(-1) / E4M3_MAX).clamp(min=tiny)
+    # a quotient rounded once: dividing by a Python number would multiply by its reciprocal
+    s = (b.abs().amax(-1) / torch.full((), E4M3_MAX, device=x.device)).clamp(min=tiny)
     q = (b / s[..., None]).reshape(x.shape[0], -1)[:, :x.shape[1]]
     return q.to(torch.float8_e4m3fn), s.t().contiguous()
 
