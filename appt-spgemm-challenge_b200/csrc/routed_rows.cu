@@ -1,0 +1,302 @@
+// Dense rows to the experts' order and back: the products of the routing matrix R (tokens x
+// sorted rows, weights as entries) with dense matrices.
+//
+//   dispatch      Y = R^T X          Y[row(p)] = w[p] X[p / k]
+//   combine       Y = R H            Y[t] = sum_j w[t,j] H[row(t,j)]
+//   combine_grad  dH = R^T dY, and the sampled product dw[p] = <dY[p / k], H[row(p)]>
+//
+// All are bound by memory: a few operations per element. Each goes by tokens, so that a token's
+// row is read (or written) once for its k pairs, and each thread moves 16-byte pieces.
+#include <cuda_runtime.h>
+#include "common.cuh"
+#include "experts.h"
+#include "values.cuh"
+
+namespace appt {
+namespace {
+
+constexpr int kThreads = 256;
+
+// What the three kernels share: `lanes` (a multiple of 32) threads per token.
+struct Shape {
+  const int* pair_row;
+  int tokens, top_k;
+  long long pieces;     // pieces of N elements per row
+  int lanes;
+};
+
+struct Place {
+  int token;            // -1: none
+  int at;               // thread's place among the token's
+};
+
+__device__ __forceinline__ Place place(const Shape& s) {
+  const int per = kThreads / s.lanes;
+  const long long t = (long long)blockIdx.x * per + threadIdx.x / s.lanes;
+  return Place{t < s.tokens ? (int)t : -1, (int)threadIdx.x % s.lanes};
+}
+
+// Rows (-1: dropped or out of range) of up to 32 pairs of a token, one per lane.
+__device__ __forceinline__ int lane_row(const Shape& s, int token, int j0, long long rows) {
+  const int j = j0 + (threadIdx.x & 31);
+  const int r = j < s.top_k ? s.pair_row[(long long)token * s.top_k + j] : -1;
+  return r >= 0 && r < rows ? r : -1;
+}
+
+template <typename A>
+__device__ __forceinline__ A lane_weight(const Shape& s, const A* w, int token, int j0, int row) {
+  return w && row >= 0 ? w[(long long)token * s.top_k + j0 + (threadIdx.x & 31)] : A(1);
+}
+
+template <typename T, int N>
+__global__ void __launch_bounds__(kThreads)
+    dispatch_kernel(Shape s, const T* __restrict__ x, long long ldx,
+                    const typename Value<T>::Acc* __restrict__ w, T* __restrict__ y, long long ldy,
+                    long long rows) {
+  using A = typename Value<T>::Acc;
+  using P = Pack<T, N>;
+  constexpr int U = 4;
+  const Place me = place(s);
+  if (me.token < 0) return;   // whole warps
+  const P* px = (const P*)(x + me.token * ldx);
+  for (long long base = (long long)blockIdx.y * s.lanes * U; base < s.pieces;
+       base += (long long)gridDim.y * s.lanes * U) {
+    P v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long c = base + me.at + (long long)u * s.lanes;
+      if (c < s.pieces) v[u] = px[c];
+    }
+    for (int j0 = 0; j0 < s.top_k; j0 += 32) {
+      const int mine = lane_row(s, me.token, j0, rows);
+      const A wmine = lane_weight(s, w, me.token, j0, mine);
+      for (int j = 0; j < 32 && j0 + j < s.top_k; ++j) {
+        const int row = __shfl_sync(kFull, mine, j);
+        const A wj = __shfl_sync(kFull, wmine, j);
+        if (row < 0) continue;
+        P* py = (P*)(y + row * ldy);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const long long c = base + me.at + (long long)u * s.lanes;
+          if (c >= s.pieces) continue;
+          P o = v[u];
+          if (w) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) o.v[i] = Value<T>::down(wj * Value<T>::up(v[u].v[i]));
+          }
+          py[c] = o;
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int N>
+__global__ void __launch_bounds__(kThreads)
+    combine_kernel(Shape s, const T* __restrict__ h, long long ldh, long long rows,
+                   const typename Value<T>::Acc* __restrict__ w, T* __restrict__ y,
+                   long long ldy) {
+  using A = typename Value<T>::Acc;
+  using P = Pack<T, N>;
+  constexpr int J = 4;   // rows in flight
+  const Place me = place(s);
+  if (me.token < 0) return;
+  P* py = (P*)(y + me.token * ldy);
+  for (long long base = (long long)blockIdx.y * s.lanes; base < s.pieces;
+       base += (long long)gridDim.y * s.lanes) {
+    const long long c = base + me.at;
+    A sum[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum[i] = A(0);
+    for (int j0 = 0; j0 < s.top_k; j0 += 32) {
+      const int mine = lane_row(s, me.token, j0, rows);
+      const A wmine = lane_weight(s, w, me.token, j0, mine);
+      for (int j = 0; j < 32 && j0 + j < s.top_k; j += J) {
+        P v[J];
+        int row[J];
+        A wj[J];
+#pragma unroll
+        for (int u = 0; u < J; ++u) {
+          row[u] = __shfl_sync(kFull, mine, (j + u) & 31);   // lanes past top_k hold -1
+          wj[u] = __shfl_sync(kFull, wmine, (j + u) & 31);
+          if (row[u] >= 0 && c < s.pieces) v[u] = ((const P*)(h + row[u] * ldh))[c];
+        }
+        if (c < s.pieces) {
+#pragma unroll
+          for (int u = 0; u < J; ++u) {
+            if (row[u] < 0) continue;
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum[i] += wj[u] * Value<T>::up(v[u].v[i]);
+          }
+        }
+      }
+    }
+    if (c < s.pieces) {
+      P o;
+#pragma unroll
+      for (int i = 0; i < N; ++i) o.v[i] = Value<T>::down(sum[i]);
+      py[c] = o;
+    }
+  }
+}
+
+// The dot products of a token's pairs go over its whole row: all of the row's columns belong to
+// one group of threads, J pairs at a time, and are summed in a fixed order (over a thread's
+// pieces, over the lanes, over the warps).
+template <typename T, int N>
+__global__ void __launch_bounds__(kThreads)
+    combine_grad_kernel(Shape s, const T* __restrict__ dy, long long ldy, const T* __restrict__ h,
+                        long long ldh, long long rows,
+                        const typename Value<T>::Acc* __restrict__ w, T* __restrict__ dh,
+                        long long lddh, typename Value<T>::Acc* __restrict__ dw) {
+  using A = typename Value<T>::Acc;
+  using P = Pack<T, N>;
+  constexpr int J = 4;
+  __shared__ A part[kThreads / 32][J];
+  const Place me = place(s);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int warps = s.lanes / 32, first = warp / warps * warps;
+  const long long token = me.token < 0 ? 0 : me.token;
+  const P* py = (const P*)(dy + token * ldy);
+  for (int j0 = 0; j0 < s.top_k; j0 += J) {
+    int row[J];
+    A wj[J], dot[J];
+#pragma unroll
+    for (int u = 0; u < J; ++u) {
+      const long long p = token * s.top_k + j0 + u;
+      row[u] = me.token >= 0 && j0 + u < s.top_k ? s.pair_row[p] : -1;
+      if (row[u] >= rows) row[u] = -1;
+      wj[u] = w && row[u] >= 0 ? w[p] : A(1);
+      dot[u] = A(0);
+    }
+    if (me.token >= 0) {
+      for (long long c = me.at; c < s.pieces; c += s.lanes) {
+        const P g = py[c];
+        P v[J];
+#pragma unroll
+        for (int u = 0; u < J; ++u)
+          if (dw && row[u] >= 0) v[u] = ((const P*)(h + row[u] * ldh))[c];
+#pragma unroll
+        for (int u = 0; u < J; ++u) {
+          if (row[u] < 0) continue;
+          if (dw) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+              dot[u] += Value<T>::up(g.v[i]) * Value<T>::up(v[u].v[i]);
+          }
+          if (dh) {
+            P o;
+#pragma unroll
+            for (int i = 0; i < N; ++i) o.v[i] = Value<T>::down(wj[u] * Value<T>::up(g.v[i]));
+            ((P*)(dh + row[u] * lddh))[c] = o;
+          }
+        }
+      }
+    }
+    if (!dw) continue;
+#pragma unroll
+    for (int u = 0; u < J; ++u) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) dot[u] += __shfl_xor_sync(kFull, dot[u], o);
+      if (lane == 0) part[warp][u] = dot[u];
+    }
+    __syncthreads();
+    if (me.token >= 0 && me.at < J && j0 + me.at < s.top_k) {
+      A sum = A(0);
+      for (int k = 0; k < warps; ++k) sum += part[first + k][me.at];
+      dw[token * s.top_k + j0 + me.at] = sum;
+    }
+    __syncthreads();
+  }
+}
+
+bool wide(const DenseView& m, int bytes) {
+  return (uintptr_t)m.data % 16 == 0 && m.ld * bytes % 16 == 0;
+}
+
+Shape shape_for(const RoutesView& r, long long pieces) {
+  Shape s{r.pair_row, r.tokens, r.top_k, pieces, 32};
+  while (s.lanes < kThreads && s.lanes < pieces) s.lanes *= 2;
+  return s;
+}
+
+dim3 grid_for(const Shape& s, long long per_cta_pieces) {
+  const int per = kThreads / s.lanes;
+  const long long y = (s.pieces + per_cta_pieces - 1) / per_cta_pieces;
+  return dim3((s.tokens + per - 1) / per, (unsigned)(y > 65535 ? 65535 : y));
+}
+
+// f(T{}, N): N elements per piece, 16 bytes where every row starts and ends on 16 bytes.
+template <typename F>
+void by_type(int type, long long cols, bool vec, F&& f) {
+  switch (type) {
+    case kF64:
+      if (vec && cols % 2 == 0) f(double(), std::integral_constant<int, 2>());
+      else f(double(), std::integral_constant<int, 1>());
+      break;
+    case kF32:
+      if (vec && cols % 4 == 0) f(float(), std::integral_constant<int, 4>());
+      else f(float(), std::integral_constant<int, 1>());
+      break;
+    case kF16:
+      if (vec && cols % 8 == 0) f(__half(), std::integral_constant<int, 8>());
+      else f(__half(), std::integral_constant<int, 1>());
+      break;
+    default:
+      if (vec && cols % 8 == 0) f(__nv_bfloat16(), std::integral_constant<int, 8>());
+      else f(__nv_bfloat16(), std::integral_constant<int, 1>());
+  }
+}
+
+int bytes_of(int type) { return type == kF64 ? 8 : type == kF32 ? 4 : 2; }
+
+}  // namespace
+
+int launch_dispatch(const RoutesView& r, const DenseView& x, const void* w, const DenseView& y,
+                    cudaStream_t s) {
+  if (r.tokens == 0 || x.cols == 0 || y.rows == 0) return 0;
+  const int b = bytes_of(x.type);
+  by_type(x.type, x.cols, wide(x, b) && wide(y, b), [&](auto t, auto n) {
+    using T = decltype(t);
+    constexpr int N = decltype(n)::value;
+    const Shape sh = shape_for(r, x.cols / N);
+    launch(nullptr, dispatch_kernel<T, N>, grid_for(sh, sh.lanes * 4), kThreads, 0, s, sh,
+           (const T*)x.data, x.ld, (const typename Value<T>::Acc*)w, (T*)y.data, y.ld, y.rows);
+  });
+  return 1;
+}
+
+int launch_combine(const RoutesView& r, const DenseView& h, const void* w, const DenseView& y,
+                   cudaStream_t s) {
+  if (r.tokens == 0 || y.cols == 0) return 0;
+  const int b = bytes_of(h.type);
+  by_type(h.type, h.cols, wide(h, b) && wide(y, b), [&](auto t, auto n) {
+    using T = decltype(t);
+    constexpr int N = decltype(n)::value;
+    const Shape sh = shape_for(r, h.cols / N);
+    launch(nullptr, combine_kernel<T, N>, grid_for(sh, sh.lanes), kThreads, 0, s, sh,
+           (const T*)h.data, h.ld, h.rows, (const typename Value<T>::Acc*)w, (T*)y.data, y.ld);
+  });
+  return 1;
+}
+
+int launch_combine_grad(const RoutesView& r, const DenseView& dy, const DenseView* h, const void* w,
+                        const DenseView* dh, void* dw, cudaStream_t s) {
+  if (r.tokens == 0 || (dy.cols == 0 && !dw)) return 0;
+  const int b = bytes_of(dy.type);
+  const bool vec = wide(dy, b) && (!h || wide(*h, b)) && (!dh || wide(*dh, b));
+  by_type(dy.type, dy.cols, vec, [&](auto t, auto n) {
+    using T = decltype(t);
+    using A = typename Value<T>::Acc;
+    constexpr int N = decltype(n)::value;
+    const Shape sh = shape_for(r, dy.cols / N);
+    const int per = kThreads / sh.lanes;
+    launch(nullptr, combine_grad_kernel<T, N>, (r.tokens + per - 1) / per, kThreads, 0, s, sh,
+           (const T*)dy.data, dy.ld, h ? (const T*)h->data : nullptr, h ? h->ld : 0,
+           h ? h->rows : dh->rows, (const A*)w, dh ? (T*)dh->data : nullptr, dh ? dh->ld : 0,
+           (A*)dw);
+  });
+  return 1;
+}
+
+}  // namespace appt

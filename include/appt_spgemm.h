@@ -293,6 +293,118 @@ int appt_comm_spgemm(appt_comm *comm, const appt_csr *A_block, const appt_csr *B
                      const appt_options *opt, appt_csr_out *C_block, int64_t *block_offsets,
                      appt_stats *stats);
 
+/* ------------------------------------------------------------------------------------------
+ * Routed products: a sparse matrix with top_k entries per row times dense matrices.
+ *
+ * The choice of top_k of `experts` experts for every token is a sparse tokens x experts matrix.
+ * These calls sort its entries by expert (its transpose), take dense rows to that order and back
+ * (its products with dense matrices, and their gradients), quantise rows to 8 bits by blocks of
+ * 128 columns, and multiply the sorted rows by each expert's own matrix. No counterpart in the
+ * reference.
+ *
+ * A pair is one (token, choice): pair p = token * top_k + choice. Sorted rows 0 .. kept - 1 hold
+ * the kept pairs in order of (expert, pair); buffers of sorted rows usually have room for all
+ * tokens * top_k pairs, and rows behind the last kept one are left as they were.
+ *
+ * All data is device memory of `device`, owned by the caller; a pointer of the host or of another
+ * device is refused. The calls are asynchronous on `stream` (a cudaStream_t of that device; NULL
+ * = its default stream), allocate nothing, read nothing back, may be captured into CUDA graphs
+ * and may run at the same time on different streams. The caller's current device is kept.
+ * Outputs must not overlap inputs or each other. Results do not depend on scheduling: the same
+ * inputs give the same bits.
+ * ---------------------------------------------------------------------------------------- */
+#define APPT_F64 0
+#define APPT_F32 1
+#define APPT_F16 2
+#define APPT_BF16 3
+#define APPT_E4M3 4 /* 8 bits: 4 exponent, 3 mantissa, largest value 448, no infinities */
+#define APPT_I32 5
+#define APPT_I64 6
+
+typedef struct appt_dense { /* row-major dense matrix in device memory */
+  int64_t rows, cols;
+  int64_t ld;       /* elements from one row to the next, >= cols (ignored with fewer than 2 rows) */
+  void *data;
+  int32_t type;     /* APPT_F64 .. APPT_I64 */
+  int32_t reserved; /* 0 */
+} appt_dense;
+
+typedef struct appt_routes { /* where each pair went, as appt_route fills it */
+  int64_t tokens;
+  int32_t top_k;
+  int32_t reserved;        /* 0 */
+  const int32_t *pair_row; /* tokens * top_k: the pair's sorted row; a value outside the row
+                              matrix (-1) is a dropped pair, which is neither read nor written */
+} appt_routes;
+
+typedef struct appt_scaled { /* values in 8 bits with one scale per row and block of 128 columns */
+  appt_dense q;     /* APPT_E4M3 */
+  float *scale;     /* scale[b * scale_ld + r] belongs to row r, columns 128 b .. 128 b + 127 */
+  int64_t scale_ld; /* >= q.rows */
+} appt_scaled;
+
+typedef struct appt_blocks { /* `groups` matrices in 8 bits, one scale per block of 128 x 128 */
+  int64_t groups, rows, cols;
+  int64_t ld;           /* elements from one row to the next: a multiple of 16, >= cols */
+  int64_t group_stride; /* elements from one matrix to the next: a multiple of 16 */
+  const void *data;     /* APPT_E4M3, 16-byte aligned */
+  const float *scale;   /* [groups][ceil(rows / 128)][ceil(cols / 128)], contiguous */
+} appt_blocks;
+
+#define APPT_MAX_EXPERTS 1024
+
+/* Bytes of device workspace that appt_route needs for these sizes (0 for invalid ones). The
+ * contents need not be initialised and are not kept: calls that may run at the same time (two
+ * streams, two captured graphs) need one workspace each. */
+size_t appt_route_workspace(int64_t tokens, int32_t top_k, int64_t experts);
+/* Sorts the pairs by expert, stably. ids: tokens x top_k, APPT_I32 or APPT_I64; an id outside
+ * [0, experts) drops its pair. Fills expert_ptr (experts + 1: expert e has the sorted rows
+ * expert_ptr[e] .. expert_ptr[e + 1] - 1), row_pair (room for tokens * top_k; the kept rows are
+ * written) and pair_row (tokens * top_k; -1 for dropped pairs). tokens * top_k < 2^31, experts
+ * <= APPT_MAX_EXPERTS. (expert_ptr, row_pair) is the CSR form of the transposed routing. */
+int appt_route(const appt_dense *ids, int64_t experts, int32_t *expert_ptr, int32_t *row_pair,
+               int32_t *pair_row, void *workspace, size_t workspace_bytes, int32_t device,
+               void *stream);
+/* Y[pair_row[p]] = weights[p] * X[p / top_k] for every kept pair (weights NULL: a copy of the
+ * bits). X: tokens rows; Y: sorted rows; one type, F64, F32, F16 or BF16. weights: tokens x
+ * top_k, contiguous, F32 (F64 with F64 data). The gradient of X is appt_combine of Y's gradient
+ * with the same weights, that of the weights appt_combine_grad(dY := X, H := Y's gradient,
+ * dH := NULL). */
+int appt_dispatch(const appt_routes *routes, const appt_dense *X, const void *weights,
+                  const appt_dense *Y, int32_t device, void *stream);
+/* Y[t] = sum over j of weights[t, j] * H[pair_row[t, j]], in order of j, summed in F32 (F64 with
+ * F64 data) and rounded once; a token without kept pairs gets zeros. Types and weights as
+ * appt_dispatch. */
+int appt_combine(const appt_routes *routes, const appt_dense *H, const void *weights,
+                 const appt_dense *Y, int32_t device, void *stream);
+/* Gradient of appt_combine: dH[pair_row[p]] = weights[p] * dY[p / top_k] for kept pairs, and
+ * dweights[p] = <dY[p / top_k], H[pair_row[p]]> summed in F32 (F64), 0 for dropped pairs.
+ * dH or dweights may be NULL (not wanted); H may be NULL when dweights is. */
+int appt_combine_grad(const appt_routes *routes, const appt_dense *dY, const appt_dense *H,
+                      const void *weights, const appt_dense *dH, void *dweights, int32_t device,
+                      void *stream);
+
+#define APPT_GATE_NONE 0
+#define APPT_GATE_SILU 1 /* values are silu(X[:, :n]) * X[:, n:], n = Q's columns, X has 2 n */
+
+/* Rows to 8 bits: for each row and block of 128 columns, scale = max(|largest value| / 448,
+ * smallest normal float), q = value / scale rounded to nearest even. A NaN or infinity makes its
+ * block's scale NaN or infinite. X: F32, F16 or BF16. rows_ptr (device, may be NULL: all): only
+ * rows 0 .. *rows_ptr - 1 are read and written, e.g. expert_ptr + experts. */
+int appt_quantize(const appt_dense *X, int32_t gate, const int32_t *rows_ptr,
+                  const appt_scaled *Q, int32_t device, void *stream);
+/* appt_quantize of X's rows, written to each kept pair's sorted row (dispatch in 8 bits). */
+int appt_dispatch_quantize(const appt_routes *routes, const appt_dense *X, const appt_scaled *Q,
+                           int32_t device, void *stream);
+/* Y[r, n] = sum over blocks b of A.scale[b, r] * W.scale[g, n / 128, b] * (sum over the block's
+ * columns k of A[r, k] * W[g, n, k]) for the rows r of every group g: group_ptr[g] .. group_ptr[g +
+ * 1] - 1 (groups + 1 device entries, ascending, e.g. expert_ptr; NULL with one group: all rows).
+ * Rows of no group are left as they were. Y: F32, F16 or BF16, rows x W.rows; sums in F32,
+ * rounded once. A.q.ld must be a multiple of 16 and A.q.data 16-byte aligned; any number of
+ * columns. */
+int appt_scaled_product(const appt_scaled *A, const appt_blocks *W, const int32_t *group_ptr,
+                        const appt_dense *Y, int32_t device, void *stream);
+
 const char *appt_last_error(void);
 int appt_device_count(void);
 /* Device memory that the library keeps cached for later calls (freed temporaries and released
