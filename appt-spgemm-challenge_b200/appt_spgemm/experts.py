@@ -76,6 +76,7 @@ def _lib() -> ct.CDLL:
         fn.argtypes, fn.restype = argtypes, ct.c_int
     lib.appt_route_workspace.argtypes = [ct.c_int64, ct.c_int32, ct.c_int64]
     lib.appt_route_workspace.restype = ct.c_size_t
+    lib.appt_scaled_product_status.argtypes, lib.appt_scaled_product_status.restype = [dev], ct.c_int
     _ready = lib
     return lib
 
@@ -314,3 +315,9 @@ class ScaledProduct(_Call):
         mw = BlocksArg(groups, n, k, ld, step, d.ptr, sw)
         ptr = self._flat(expert_ptr, "expert_ptr", ("i32",), groups + 1)
         self._set(ma, mw, ptr, self._matrix(y, "y"))
+
+
+def check_products(device: int = 0) -> None:
+    """Waits for the device and raises if a ScaledProduct on it has given up a wait since the last
+    check (its y is then incomplete)."""
+    _check(_lib().appt_scaled_product_status(device), "appt_scaled_product_status")

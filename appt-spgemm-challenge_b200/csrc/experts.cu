@@ -421,4 +421,14 @@ int appt_scaled_product(const appt_scaled* A, const appt_blocks* W, const int32_
   });
 }
 
+int appt_scaled_product_status(int32_t device) {
+  return guarded("appt_scaled_product_status", [&] {
+    OnDevice on(device);
+    check_cuda(cudaDeviceSynchronize(), "cudaDeviceSynchronize");
+    int gave_up = 0;
+    check_cuda((cudaError_t)scaled_product_status(&gave_up), "reading the status");
+    if (gave_up) refuse("a product gave up a wait", kErrDevice);
+  });
+}
+
 }  // extern "C"

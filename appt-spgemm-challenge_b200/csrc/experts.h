@@ -13,12 +13,12 @@ struct LaunchFailed {   // thrown by launch(), turned into a status at the C ent
   cudaError_t error;
 };
 
-// kernel<<<grid, block, smem, s>>>(args...), with the launch's own status (an error that an
+// kernel<<<grid, block, smem, s>>>(args...) in clusters of `cluster` CTAs, with the launch's own status (an error that an
 // earlier call of the program left behind is not taken for it). The opt-in to more than 48 KB of
 // shared memory is per device and kept in *opted, a bit per device.
 template <typename... P, typename... A>
 void launch(std::atomic<unsigned long long>* opted, void (*kernel)(P...), dim3 grid, dim3 block,
-            size_t smem, cudaStream_t s, A... args) {
+            size_t smem, cudaStream_t s, int cluster, A... args) {
   cudaError_t e = cudaSuccess;
   if (smem > 48 * 1024) {
     int dev = 0;
@@ -40,6 +40,12 @@ void launch(std::atomic<unsigned long long>* opted, void (*kernel)(P...), dim3 g
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
     e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
   }
   if (e != cudaSuccess) {
@@ -93,5 +99,7 @@ int launch_quantize(const DenseView& x, bool gated, const int* rows_ptr, const R
 // scaled_product.cu
 int launch_scaled_product(const ScaledView& a, const BlocksView& w, const int* group_ptr,
                           const DenseView& y, int sms, cudaStream_t s);
+// Reads and clears the current device's record of products that gave up a wait (a cudaError_t).
+int scaled_product_status(int* gave_up);
 
 }  // namespace appt

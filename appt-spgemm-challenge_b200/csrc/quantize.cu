@@ -126,13 +126,13 @@ void quantize(const DenseView& x, bool gated, const int* rows_ptr, const RoutesV
   const dim3 grid((unsigned)(ctas < (1 << 20) ? ctas : 1 << 20));
   const T* p = (const T*)x.data;
   if (routes)
-    launch(nullptr, quantize_kernel<T, false, true>, grid, kThreads, 0, s, p, x.ld, xvec, x.rows,
+    launch(nullptr, quantize_kernel<T, false, true>, grid, kThreads, 0, s, 1, p, x.ld, xvec, x.rows,
            nullptr, routes->pair_row, routes->top_k, o);
   else if (gated)
-    launch(nullptr, quantize_kernel<T, true, false>, grid, kThreads, 0, s, p, x.ld, xvec, x.rows,
+    launch(nullptr, quantize_kernel<T, true, false>, grid, kThreads, 0, s, 1, p, x.ld, xvec, x.rows,
            rows_ptr, nullptr, 1, o);
   else
-    launch(nullptr, quantize_kernel<T, false, false>, grid, kThreads, 0, s, p, x.ld, xvec, x.rows,
+    launch(nullptr, quantize_kernel<T, false, false>, grid, kThreads, 0, s, 1, p, x.ld, xvec, x.rows,
            rows_ptr, nullptr, 1, o);
 }
 

@@ -139,9 +139,9 @@ int route(const DenseView& v, int experts, int* expert_ptr, int* row_pair, int* 
   const int chunks = chunks_for(pairs);
   const int chunk = (int)(((long long)pairs + chunks - 1) / chunks);
   if (chunks > 1)
-    launch(nullptr, route_count_kernel<Id>, chunks, kThreads, experts * sizeof(int), s, ids, chunk,
+    launch(nullptr, route_count_kernel<Id>, chunks, kThreads, experts * sizeof(int), s, 1, ids, chunk,
            counts);
-  launch(&opted, route_place_kernel<Id>, chunks, kThreads, kWarps * experts * sizeof(int), s, ids,
+  launch(&opted, route_place_kernel<Id>, chunks, kThreads, kWarps * experts * sizeof(int), s, 1, ids,
          chunk, counts, expert_ptr, row_pair, pair_row);
   return chunks > 1 ? 2 : 1;
 }

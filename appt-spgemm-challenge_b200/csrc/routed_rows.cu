@@ -260,7 +260,7 @@ int launch_dispatch(const RoutesView& r, const DenseView& x, const void* w, cons
     using T = decltype(t);
     constexpr int N = decltype(n)::value;
     const Shape sh = shape_for(r, x.cols / N);
-    launch(nullptr, dispatch_kernel<T, N>, grid_for(sh, sh.lanes * 4), kThreads, 0, s, sh,
+    launch(nullptr, dispatch_kernel<T, N>, grid_for(sh, sh.lanes * 4), kThreads, 0, s, 1, sh,
            (const T*)x.data, x.ld, (const typename Value<T>::Acc*)w, (T*)y.data, y.ld, y.rows);
   });
   return 1;
@@ -274,7 +274,7 @@ int launch_combine(const RoutesView& r, const DenseView& h, const void* w, const
     using T = decltype(t);
     constexpr int N = decltype(n)::value;
     const Shape sh = shape_for(r, h.cols / N);
-    launch(nullptr, combine_kernel<T, N>, grid_for(sh, sh.lanes), kThreads, 0, s, sh,
+    launch(nullptr, combine_kernel<T, N>, grid_for(sh, sh.lanes), kThreads, 0, s, 1, sh,
            (const T*)h.data, h.ld, h.rows, (const typename Value<T>::Acc*)w, (T*)y.data, y.ld);
   });
   return 1;
@@ -291,7 +291,7 @@ int launch_combine_grad(const RoutesView& r, const DenseView& dy, const DenseVie
     constexpr int N = decltype(n)::value;
     const Shape sh = shape_for(r, dy.cols / N);
     const int per = kThreads / sh.lanes;
-    launch(nullptr, combine_grad_kernel<T, N>, (r.tokens + per - 1) / per, kThreads, 0, s, sh,
+    launch(nullptr, combine_grad_kernel<T, N>, (r.tokens + per - 1) / per, kThreads, 0, s, 1, sh,
            (const T*)dy.data, dy.ld, h ? (const T*)h->data : nullptr, h ? h->ld : 0,
            h ? h->rows : dh->rows, (const A*)w, dh ? (T*)dh->data : nullptr, dh ? dh->ld : 0,
            (A*)dw);

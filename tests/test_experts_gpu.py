@@ -520,6 +520,7 @@ def test_scaled_product(case, dtype):
     y = base[:, :n]
     ex.ScaledProduct(a, sa, w, sw, y, expert_ptr=dptr).run(stream())
     want, size = product_oracle(a, sa, w, sw, ptr)
+    ex.check_products()
     close(y[ptr[0]:ptr[-1]], want[ptr[0]:ptr[-1]],
           product_tol(want, size, k, dtype)[ptr[0]:ptr[-1]])
     assert (base[:, n:] == 9.0).all()
