@@ -23,7 +23,7 @@
 // timing.
 #include <cuda.h>
 #include <cuda_runtime.h>
-#include <mutex>
+#include <climits>
 #include "common.cuh"
 #include "experts.h"
 #include "tcgen05.cuh"
@@ -38,13 +38,13 @@ __device__ int g_product_gave_up;
 
 namespace {
 
-constexpr int kThreads = 384;
 constexpr int kLanes = 128;                 // rows of a tile's first operand
 constexpr int kTileBytes = kLanes * kScaleBlock;
 constexpr int kScaleStages = 8;
 constexpr int kMaxStages = 10;
 constexpr int kMaxBuffers = 4;
 constexpr int kSharedMax = 227 * 1024;
+constexpr int kOutRow = 64, kOutWarp = 32 * kOutRow;   // a warp's piece of Y on its way out
 
 struct Params {
   const float* sa;
@@ -75,14 +75,17 @@ struct Shape {
   static constexpr int kStageBytes = kTileBytes + kCols * kScaleBlock;
   static constexpr int kRowTile = kSwap ? kCols : kLanes;      // rows of Y per tile
   static constexpr int kNTile = kSwap ? kLanes : kCols;        // columns of Y per tile
-  static constexpr int kWScales = (kNTile + kScaleBlock - 1) / kScaleBlock;
-  static constexpr int kScaleFloats = kRowTile + 4;            // rows, then up to 2 of the weights
+  static constexpr int kScaleFloats = kSwap ? kCols + 4 : 0;   // the rows', then the weights'
   static constexpr int kBuffers = 512 / kCols < kMaxBuffers ? 512 / kCols : kMaxBuffers;
-  // 128 sums a thread: the adding warps take registers of the other four. 128 x 56 + 256 x 216 =
-  // 62,464 of the 384 x 168 = 64,512 that the launch holds.
+  // 128 sums a thread: the adding warps take registers of the other four. 128 x 56 + 256 x 224 =
+  // 64,512, the 384 x 168 that the launch holds.
   static constexpr bool kMoveRegs = kCols == 256;
   static constexpr int kTmemColumns = kBuffers * kCols < 32 ? 32 : kBuffers * kCols;
-  static constexpr int kFixedBytes = (int)sizeof(Groups) + (int)sizeof(Barriers) + 64 +
+  static constexpr int kGroups = 2;               // adding warpgroups
+  static constexpr int kThreads = 128 + 128 * kGroups;
+  static constexpr int kPart = kCols / kGroups;                // columns of a warpgroup
+  static constexpr int kOutBytes = kSwap ? 0 : 4 * kGroups * kOutWarp;
+  static constexpr int kFixedBytes = kOutBytes + (int)sizeof(Groups) + (int)sizeof(Barriers) + 64 +
                                      kScaleStages * kScaleFloats * 4 + 1024;
   static constexpr int kStages = (kSharedMax - kFixedBytes) / kStageBytes < kMaxStages
                                      ? (kSharedMax - kFixedBytes) / kStageBytes
@@ -96,22 +99,39 @@ __device__ __forceinline__ void store_one(const Params& p, long long at, float v
   else ((__nv_bfloat16*)p.y)[at] = __float2bfloat16_rn(v);
 }
 
-// 8 neighbouring values of a row
-__device__ __forceinline__ void store_eight(const Params& p, long long at, const float* v) {
-  if (p.type == kF32) {
-    float4* d = (float4*)((float*)p.y + at);
-    d[0] = make_float4(v[0], v[1], v[2], v[3]);
-    d[1] = make_float4(v[4], v[5], v[6], v[7]);
-  } else if (p.type == kF16) {
-    Pack<__half, 8> o;
+// A warp's 32 rows x N columns of Y, a row per thread, by way of shared memory: 64 bytes of each
+// row at a time, so that a store writes 8 rows' whole 64 bytes instead of 16 bytes of 32 rows.
+// Pieces of 16 bytes change places by the row, which spreads both accesses over all banks.
+template <typename T, int N>
+__device__ __forceinline__ void write_rows(const Params& p, char* piece, const float* v, int row0,
+                                           int row_end, int n0) {
+  constexpr int kPer = 16 / sizeof(T), kCols = kOutRow / sizeof(T);
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o.v[i] = __float2half_rn(v[i]);
-    *(Pack<__half, 8>*)((__half*)p.y + at) = o;
-  } else {
-    Pack<__nv_bfloat16, 8> o;
+  for (int c0 = 0; c0 < N; c0 += kCols) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o.v[i] = __float2bfloat16_rn(v[i]);
-    *(Pack<__nv_bfloat16, 8>*)((__nv_bfloat16*)p.y + at) = o;
+    for (int j = 0; j < 4; ++j) {
+      Pack<T, kPer> o;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) o.v[i] = Value<T>::down(v[c0 + j * kPer + i]);
+      *(Pack<T, kPer>*)(piece + lane * kOutRow + (j ^ (lane >> 1 & 3)) * 16) = o;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = k * 8 + lane / 4, j = lane & 3, n = n0 + c0 + j * kPer;
+      const Pack<T, kPer> o = *(Pack<T, kPer>*)(piece + r * kOutRow + (j ^ (r >> 1 & 3)) * 16);
+      T* y = (T*)p.y + (row0 + r) * p.ldy + n;
+      if (row0 + r >= row_end || n >= p.n) continue;
+      if (n + kPer <= p.n) {
+        *(Pack<T, kPer>*)y = o;
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          if (n + i < p.n) y[i] = o.v[i];
+      }
+    }
+    __syncwarp();
   }
 }
 
@@ -119,7 +139,7 @@ __device__ __forceinline__ void store_eight(const Params& p, long long at, const
 // groups never overlap and never leave the operands, whatever the offsets are.
 template <int kRowTile>
 __device__ void fill_groups(const Params& p, Groups* t) {
-  for (int g = threadIdx.x; g <= p.groups; g += kThreads)
+  for (int g = threadIdx.x; g <= p.groups; g += blockDim.x)
     t->row[g] = p.group_ptr ? min(max(p.group_ptr[g], 0), p.rows) : (g ? p.rows : 0);
   __syncthreads();
   if (threadIdx.x < 32) {
@@ -154,35 +174,34 @@ struct Tile {
 };
 
 template <int kRowTile, int kNTile>
-__device__ __forceinline__ Tile tile_at(const Params& p, const Groups* t, long long i,
-                                        int n_tiles) {
-  const int rt = (int)(i / n_tiles);
+__device__ __forceinline__ Tile tile_at(const Params& p, const Groups* t, int i, int n_tiles) {
+  const int rt = i / n_tiles;
   int lo = 0, hi = p.groups - 1;   // the last group whose first tile is <= rt
   while (lo < hi) {
     const int mid = (lo + hi + 1) / 2;
     if (t->tile[mid] <= rt) lo = mid; else hi = mid - 1;
   }
   return Tile{lo, t->row[lo] + (rt - t->tile[lo]) * kRowTile, t->row[lo + 1],
-              (int)(i % n_tiles) * kNTile};
+              (i - rt * n_tiles) * kNTile};
 }
 
 template <bool kSwap, int kCols>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_a,
                    const __grid_constant__ CUtensorMap map_w, const Params p, int splits) {
   using S = Shape<kSwap, kCols>;
-  constexpr int kHalf = kCols / 2;            // columns of a warpgroup
-  constexpr int kChunk = kHalf < 32 ? kHalf : 32;
+  constexpr int kPart = S::kPart;             // columns of a warpgroup
   extern __shared__ char raw[];
   char* base = (char*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
-  Groups* groups = (Groups*)(base + S::kStages * S::kStageBytes);
+  char* out = base + S::kStages * S::kStageBytes;
+  Groups* groups = (Groups*)(out + S::kOutBytes);
   float* scales = (float*)(groups + 1);
   Barriers* bars = (Barriers*)(((uintptr_t)(scales + kScaleStages * S::kScaleFloats) + 7) &
                                ~(uintptr_t)7);
   uint32_t* tmem_slot = (uint32_t*)(bars + 1);
   volatile int* gave_up = (volatile int*)(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(kFull, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(smem_u32(&bars->full[i]), 1);
@@ -190,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < S::kBuffers; ++i) {
       mbar_init(smem_u32(&bars->tfull[i]), 1);
-      mbar_init(smem_u32(&bars->tempty[i]), 8);
+      mbar_init(smem_u32(&bars->tempty[i]), 4 * S::kGroups);
     }
     for (int i = 0; i < kScaleStages; ++i) {
       mbar_init(smem_u32(&bars->sfull[i]), 64);
@@ -209,66 +228,75 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *tmem_slot;
 
   const int n_tiles = (p.n + S::kNTile - 1) / S::kNTile;
-  const long long tiles = (long long)groups->tile[p.groups] * n_tiles;
+  const int tiles = groups->tile[p.groups] * n_tiles;   // below 2^31: checked by the host
   const int rank = splits > 1 ? (int)cluster_rank() : 0;
-  const long long first = blockIdx.x / splits, step = gridDim.x / splits;
+  const int first = blockIdx.x / splits, step = gridDim.x / splits;
   const int kb0 = (int)((long long)p.k_blocks * rank / splits);
   const int kb1 = (int)((long long)p.k_blocks * (rank + 1) / splits);
 
   if (warp < 4) {
     if (S::kMoveRegs) regs_fewer<56>();
-    if (warp == 0 && lane == 0) {
+    if (warp == 0) {
       // ---- tiles by TMA
-      int it = 0;
+      int it = 0, st = 0;
+      uint32_t phase = 1;
       bool ok = true;
-      for (long long i = first; ok && i < tiles; i += step) {
+      for (int i = first; ok && i < tiles; i += step) {
         const Tile t = tile_at<S::kRowTile, S::kNTile>(p, groups, i, n_tiles);
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int st = it % S::kStages;
-          ok = mbar_wait(smem_u32(&bars->empty[st]), (it / S::kStages & 1) ^ 1, gave_up);
+          ok = mbar_wait(smem_u32(&bars->empty[st]), phase, gave_up);
           if (!ok) break;
           const uint32_t full = smem_u32(&bars->full[st]);
           const uint32_t at = smem_u32(base + st * S::kStageBytes);
-          mbar_expect(full, S::kStageBytes);
-          tma_load_2d(kSwap ? at + kTileBytes : at, &map_a, kb * kScaleBlock, t.row, full);
-          tma_load_3d(kSwap ? at : at + kTileBytes, &map_w, kb * kScaleBlock, t.n, t.group, full);
+          if (elect_one()) {
+            mbar_expect(full, S::kStageBytes);
+            tma_load_2d(kSwap ? at + kTileBytes : at, &map_a, kb * kScaleBlock, t.row, full);
+            tma_load_3d(kSwap ? at : at + kTileBytes, &map_w, kb * kScaleBlock, t.n, t.group, full);
+          }
+          if (++st == S::kStages) st = 0, phase ^= 1;
         }
       }
       if (!ok)   // let the loads in flight land before the CTA ends
         for (int j = max(0, it - S::kStages); j < it; ++j)
           for (int n = 0; n < kWaitTries; ++n)
             if (mbar_try(smem_u32(&bars->full[j % S::kStages]), j / S::kStages & 1)) break;
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
       // ---- products
       constexpr uint32_t idesc = instr_desc(kLanes, kCols);
-      int it = 0;
+      int st = 0, b = 0;
+      uint32_t phase = 0, bphase = 1;
       bool ok = true;
-      for (long long i = first; ok && i < tiles; i += step) {
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int st = it % S::kStages, b = it % S::kBuffers;
-          ok = mbar_wait(smem_u32(&bars->full[st]), it / S::kStages & 1, gave_up) &&
-               mbar_wait(smem_u32(&bars->tempty[b]), (it / S::kBuffers & 1) ^ 1, gave_up);
+      for (int i = first; ok && i < tiles; i += step) {
+        for (int kb = kb0; kb < kb1; ++kb) {
+          ok = mbar_wait(smem_u32(&bars->full[st]), phase, gave_up) &&
+               mbar_wait(smem_u32(&bars->tempty[b]), bphase, gave_up);
           if (!ok) break;
           fence_after();
           const uint32_t at = smem_u32(base + st * S::kStageBytes);
           const uint64_t da = smem_desc(at), db = smem_desc(at + kTileBytes);
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < kScaleBlock / 32; ++k)
-            mma_f8(tmem + b * kCols, da + 2 * k, db + 2 * k, idesc, k > 0);
-          mma_commit(smem_u32(&bars->empty[st]));
-          mma_commit(smem_u32(&bars->tfull[b]));
+            for (int k = 0; k < kScaleBlock / 32; ++k)
+              mma_f8(tmem + b * kCols, da + 2 * k, db + 2 * k, idesc, k > 0);
+            mma_commit(smem_u32(&bars->tfull[b]));
+            mma_commit(smem_u32(&bars->empty[st]));
+          }
+          __syncwarp();
+          if (++st == S::kStages) st = 0, phase ^= 1;
+          if (++b == S::kBuffers) b = 0, bphase ^= 1;
         }
       }
       // products (and their arrivals) in flight end before the CTA does
-      mma_commit(smem_u32(&bars->drain));
+      if (elect_one()) mma_commit(smem_u32(&bars->drain));
+      __syncwarp();
       for (int n = 0; n < kWaitTries; ++n)
         if (mbar_try(smem_u32(&bars->drain), 0)) break;
-    } else if (warp >= 2) {
+    } else if (kSwap) {
       // ---- scales
       const int me = threadIdx.x - 64;
       int it = 0;
       bool ok = true;
-      for (long long i = first; ok && i < tiles; i += step) {
+      for (int i = first; ok && i < tiles; i += step) {
         const Tile t = tile_at<S::kRowTile, S::kNTile>(p, groups, i, n_tiles);
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int st = it % kScaleStages;
@@ -279,13 +307,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool in = t.row + r < t.row_end;
             cp_async_4(smem_u32(s + r), p.sa + kb * p.sa_ld + (in ? t.row + r : t.row), in);
           }
-          if (me < S::kWScales) {
-            const int nb = t.n / kScaleBlock + me;
-            const bool in = nb < p.n_blocks;
-            cp_async_4(smem_u32(s + S::kRowTile + me),
-                       p.sw + ((long long)t.group * p.n_blocks + (in ? nb : 0)) * p.k_blocks + kb,
-                       in);
-          }
+          if (me == 0)
+            cp_async_4(smem_u32(s + S::kRowTile),
+                       p.sw + ((long long)t.group * p.n_blocks + t.n / kScaleBlock) * p.k_blocks + kb,
+                       true);
           cp_async_arrive(smem_u32(&bars->sfull[st]));
         }
       }
@@ -294,77 +319,155 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else {
     // ---- scaling, adding, writing
-    if (S::kMoveRegs) regs_more<216>();
+    if (S::kMoveRegs) regs_more<224>();
     const int wg = (warp - 4) / 4, quarter = warp & 3;
     const int who = quarter * 32 + lane;         // lane of the tile
-    const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16) + wg * kHalf;
+    const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16) + wg * kPart;
     int it = 0;
     bool ok = true;
-    for (long long i = first; ok && i < tiles; i += step) {
-      const Tile t = tile_at<S::kRowTile, S::kNTile>(p, groups, i, n_tiles);
-      float sum[kHalf];
+    uint64_t pairs[kPart / 2];   // sums of neighbouring columns
+    auto full_bar = [&](int n) { return smem_u32(&bars->tfull[n % S::kBuffers]); };
+    auto full_phase = [&](int n) { return (uint32_t)(n / S::kBuffers & 1); };
+    auto buffer = [&](int n) { return mine + n % S::kBuffers * kCols; };
+    auto buffer_read = [&](int n) {
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bars->tempty[n % S::kBuffers]));
+    };
+    auto clear = [&] {
 #pragma unroll
-      for (int c = 0; c < kHalf; ++c) sum[c] = 0.f;
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const int st = it % kScaleStages, b = it % S::kBuffers;
-        ok = mbar_wait(smem_u32(&bars->sfull[st]), it / kScaleStages & 1, gave_up) &&
-             mbar_wait(smem_u32(&bars->tfull[b]), it / S::kBuffers & 1, gave_up);
-        ok = __all_sync(kFull, ok);
-        if (!ok) break;
-        const float* s = scales + st * S::kScaleFloats;
-        const float sw = s[S::kRowTile + (S::kWScales > 1 ? wg : 0)];
-        const float scale = kSwap ? sw : sw * s[who];
+      for (int c = 0; c < kPart / 2; ++c) pairs[c] = 0;
+    };
+    if constexpr (!kSwap) {
+      // A thread's scales come two blocks ahead, those of its next tile before it writes this one.
+      const float *pa, *pw;
+      float a0, w0, a1, w1;
+      auto begin = [&](const Tile& t) {
+        pa = p.sa + min(t.row + who, t.row_end - 1);
+        pw = p.sw + ((long long)t.group * p.n_blocks +
+                     min((t.n + wg * kPart) / kScaleBlock, p.n_blocks - 1)) * p.k_blocks;
+        const int second = min(1, p.k_blocks - 1);
+        a0 = pa[0], w0 = pw[0];
+        a1 = pa[second * p.sa_ld], w1 = pw[second];
+      };
+      // Adds one partial tile, 16 columns at a time: the next 16 are on their way while these are
+      // added, across the end of the tile too, whose barrier is asked for 16 columns early.
+      constexpr int kChunk = 16, kChunks = kPart / kChunk;
+      static_assert(kChunks % 2 == 0, "a tile begins in the first array");
+      uint32_t part[2][kChunk];
+      auto start = [&] {
+        ok = mbar_wait(full_bar(it), full_phase(it), gave_up);
         fence_after();
-        uint32_t part[2][kChunk];
-        tmem_load(part[0], mine + b * kCols);
+        if (ok) tmem_load(part[0], buffer(it));
+      };
+      // (no copy from one pair of scales to the other: it would wait for a load in flight)
+      auto block = [&](float& a, float& w, int kb) {
+        const uint64_t scale = two(a * w, a * w);
+        const int then = min(kb + 2, p.k_blocks - 1);
+        a = pa[then * p.sa_ld], w = pw[then];
+        const bool more = kb + 1 < p.k_blocks;
+        bool ready = false;
 #pragma unroll
-        for (int c = 0; c < kHalf; c += kChunk) {
-          uint32_t(&now)[kChunk] = part[c / kChunk & 1];
+        for (int c = 0; c < kChunks; ++c) {
+          uint32_t(&now)[kChunk] = part[c & 1];
+          uint32_t(&next)[kChunk] = part[c & 1 ^ 1];
           tmem_wait(now);
-          if (c + kChunk < kHalf)
-            tmem_load(part[(c / kChunk & 1) ^ 1], mine + b * kCols + c + kChunk);
-          else {
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&bars->tempty[b]));
+          if (c + 1 < kChunks) {
+            tmem_load(next, buffer(it) + (c + 1) * kChunk);
+          } else {
+            buffer_read(it);
+            if (more) {
+              if (!__all_sync(kFull, ready))
+                ok = mbar_wait(full_bar(it + 1), full_phase(it + 1), gave_up);
+              fence_after();
+              if (ok) tmem_load(next, buffer(it + 1));
+            }
           }
+          if (c + 2 == kChunks && more) ready = mbar_try(full_bar(it + 1), full_phase(it + 1));
 #pragma unroll
-          for (int j = 0; j < kChunk; ++j) {
-            const float f = kSwap ? scale * s[wg * kHalf + c + j] : scale;
-            sum[c + j] = fmaf(__uint_as_float(now[j]), f, sum[c + j]);
-          }
+          for (int j = 0; j < kChunk; j += 2)
+            pairs[(c * kChunk + j) / 2] =
+                fma_two(now[j], now[j + 1], scale, pairs[(c * kChunk + j) / 2]);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&bars->sempty[st]));
+        ++it;
+      };
+      Tile t = {};
+      if (first < tiles) {
+        t = tile_at<S::kRowTile, S::kNTile>(p, groups, first, n_tiles);
+        begin(t);
       }
-      if (!ok) break;
-      if constexpr (kSwap) {
+      for (int i = first; i < tiles; i += step) {
+        clear();
+        start();
+        for (int kb = 0; ok && kb < p.k_blocks; kb += 2) {
+          block(a0, w0, kb);
+          if (ok && kb + 1 < p.k_blocks) block(a1, w1, kb + 1);
+        }
+        if (!ok) break;
+        const Tile done = t;
+        if (i + step < tiles) {
+          t = tile_at<S::kRowTile, S::kNTile>(p, groups, i + step, n_tiles);
+          begin(t);
+        }
+        float sum[kPart];
+#pragma unroll
+        for (int c = 0; c < kPart; c += 2) untwo(pairs[c / 2], sum[c], sum[c + 1]);
+        char* piece = out + (warp - 4) * kOutWarp;
+        const int row0 = done.row + quarter * 32, n0 = done.n + wg * kPart;
+        if (!p.vec) {
+          if (row0 + lane < done.row_end) {
+            const long long at = (row0 + lane) * p.ldy + n0;
+#pragma unroll
+            for (int c = 0; c < kPart; ++c)
+              if (n0 + c < p.n) store_one(p, at + c, sum[c]);
+          }
+        } else if (p.type == kF32) {
+          write_rows<float, kPart>(p, piece, sum, row0, done.row_end, n0);
+        } else if (p.type == kF16) {
+          write_rows<__half, kPart>(p, piece, sum, row0, done.row_end, n0);
+        } else {
+          write_rows<__nv_bfloat16, kPart>(p, piece, sum, row0, done.row_end, n0);
+        }
+      }
+    } else {
+      for (int i = first; i < tiles; i += step) {
+        const Tile t = tile_at<S::kRowTile, S::kNTile>(p, groups, i, n_tiles);
+        clear();
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int st = it % kScaleStages;
+          ok = mbar_wait(smem_u32(&bars->sfull[st]), it / kScaleStages & 1, gave_up);
+          if (!ok) break;
+          const float* s = scales + st * S::kScaleFloats;
+          const float sw = s[S::kRowTile];
+          ok = mbar_wait(full_bar(it), full_phase(it), gave_up);
+          if (!ok) break;
+          fence_after();
+          uint32_t now[kPart];
+          tmem_load(now, buffer(it));
+          tmem_wait(now);
+          buffer_read(it);
+#pragma unroll
+          for (int c = 0; c < kPart; c += 2)
+            pairs[c / 2] = fma_two(now[c], now[c + 1],
+                                   two(sw * s[wg * kPart + c], sw * s[wg * kPart + c + 1]),
+                                   pairs[c / 2]);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&bars->sempty[st]));
+        }
+        if (!ok) break;
+        float sum[kPart];
+#pragma unroll
+        for (int c = 0; c < kPart; c += 2) untwo(pairs[c / 2], sum[c], sum[c + 1]);
         if (splits > 1) {
           // the stages are free: every load has been used by a product that is done
           float* part = (float*)base;
 #pragma unroll
-          for (int c = 0; c < kHalf; ++c) part[(wg * kHalf + c) * kLanes + who] = sum[c];
+          for (int c = 0; c < kPart; ++c) part[(wg * kPart + c) * kLanes + who] = sum[c];
         } else if (t.n + who < p.n) {
 #pragma unroll
-          for (int c = 0; c < kHalf; ++c) {
-            const int r = t.row + wg * kHalf + c;
+          for (int c = 0; c < kPart; ++c) {
+            const int r = t.row + wg * kPart + c;
             if (r < t.row_end) store_one(p, r * p.ldy + t.n + who, sum[c]);
-          }
-        }
-      } else {
-        const int r = t.row + who;
-        if (r < t.row_end) {
-          const long long at = r * p.ldy + t.n + wg * kHalf;
-#pragma unroll
-          for (int c = 0; c < kHalf; c += 8) {
-            const int n = t.n + wg * kHalf + c;
-            if (p.vec && n + 8 <= p.n) {
-              store_eight(p, at + c, &sum[c]);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 8; ++j)
-                if (n + j < p.n) store_one(p, at + c + j, sum[c + j]);
-            }
           }
         }
       }
@@ -446,11 +549,12 @@ void product(const ScaledView& a, const BlocksView& w, const Params& p, int sms,
   const long long row_tiles =
       p.rows / S::kRowTile + (w.groups < p.rows ? w.groups : (long long)p.rows);
   const long long tiles = row_tiles * n_tiles;
+  if (tiles > INT_MAX - sms) throw LaunchFailed{cudaErrorInvalidValue};   // no memory holds such a Y
   int splits = 1;
   if (kSwap)
     while (splits < 8 && tiles * splits * 2 <= sms && splits * 2 <= p.k_blocks) splits *= 2;
   const long long ctas = splits > 1 ? tiles * splits : tiles < sms ? tiles : sms;
-  launch(&opted, product_kernel<kSwap, kCols>, dim3((unsigned)ctas), dim3(kThreads), S::kBytes, s,
+  launch(&opted, product_kernel<kSwap, kCols>, dim3((unsigned)ctas), dim3(S::kThreads), S::kBytes, s,
          splits, ma, mw, p, splits);
 }
 
