@@ -60,8 +60,9 @@ def _lib() -> ct.CDLL:
     if _ready is not None:
         return _ready
     lib = load()
-    vp, dev, dense = ct.c_void_p, ct.c_int32, ct.POINTER(DenseArg)
-    routes, scaled = ct.POINTER(RoutesArg), ct.POINTER(ScaledArg)
+    # structures are passed by their addresses, which _Call keeps alive: cheaper per call than byref
+    vp, dev = ct.c_void_p, ct.c_int32
+    dense = routes = scaled = blocks = vp
     sigs = {
         "appt_route": [dense, ct.c_int64, vp, vp, vp, vp, ct.c_size_t, dev, vp],
         "appt_dispatch": [routes, dense, vp, dense, dev, vp],
@@ -69,7 +70,7 @@ def _lib() -> ct.CDLL:
         "appt_combine_grad": [routes, dense, dense, vp, dense, vp, dev, vp],
         "appt_quantize": [dense, ct.c_int32, vp, scaled, dev, vp],
         "appt_dispatch_quantize": [routes, dense, scaled, dev, vp],
-        "appt_scaled_product": [scaled, ct.POINTER(BlocksArg), vp, dense, dev, vp],
+        "appt_scaled_product": [scaled, blocks, vp, dense, dev, vp],
     }
     for name, argtypes in sigs.items():
         fn = getattr(lib, name)
@@ -182,12 +183,15 @@ class _Call:
         return ScaledArg(m, s.data, s.ld)
 
     def _set(self, *args) -> None:
-        # structures go by reference; byref keeps them alive
-        self._args = tuple(ct.byref(a) if isinstance(a, ct.Structure) else a for a in args)
+        self._structures = [a for a in args if isinstance(a, ct.Structure)]
+        self._args = tuple(ct.addressof(a) if isinstance(a, ct.Structure) else a for a in args)
+        self._args += (self._device,)
 
     def run(self, stream: int | None = None):
         """Makes the call on `stream`; returns self."""
-        _check(self._fn(*self._args, self._device, stream), self._entry)
+        rc = self._fn(*self._args, stream)
+        if rc:
+            _check(rc, self._entry)
         return self
 
 

@@ -88,8 +88,8 @@ const DenseView view(const appt_dense* m, const char* name, unsigned types, int 
   v.cols = m->cols;
   v.type = m->type;
   v.ld = m->rows > 1 ? m->ld : (m->cols + 15) / 16 * 16;
-  if (m->rows > 1 && (m->ld < m->cols || m->ld >= (1ll << 40)))
-    refuse(std::string(name) + ": ld must be at least cols");
+  if (m->rows > 1 && (m->ld < m->cols || m->ld >= INT_MAX))
+    refuse(std::string(name) + ": ld must be at least cols and below 2^31 - 1");
   v.data = m->data;
   if (v.rows > 0 && v.cols > 0) {
     if (!v.data) refuse(std::string(name) + ": null data");
@@ -131,8 +131,8 @@ ScaledView view(const appt_scaled* q, const char* name, bool out, int align, Spa
   if (v.q.rows > 0 && v.q.cols > 0) {
     if (!v.scale || (uintptr_t)v.scale % 4)
       refuse(std::string(name) + ": scale is null or not aligned to 4 bytes");
-    if (blocks > 1 && (v.scale_ld < v.q.rows || v.scale_ld >= (1ll << 40)))
-      refuse(std::string(name) + ": scale_ld must be at least the rows");
+    if (blocks > 1 && (v.scale_ld < v.q.rows || v.scale_ld >= INT_MAX))
+      refuse(std::string(name) + ": scale_ld must be at least the rows and below 2^31 - 1");
   }
   if (blocks <= 1) v.scale_ld = v.q.rows;
   sp->add(name, v.q, out);
@@ -264,8 +264,8 @@ int appt_route(const appt_dense* ids, int64_t experts, int32_t* expert_ptr, int3
     check_overlap(sp);
     OnDevice on(device);
     check_resident(sp, device);
-    note_launches(launch_route(v, (int)experts, expert_ptr, row_pair, pair_row, (int*)workspace, on.sms,
-                          (cudaStream_t)stream));
+    note_launches(launch_route(v, (int)experts, expert_ptr, row_pair, pair_row, (int*)workspace,
+                               (cudaStream_t)stream));
   });
 }
 

@@ -13,6 +13,11 @@ struct LaunchFailed {   // thrown by launch(), turned into a status at the C ent
   cudaError_t error;
 };
 
+// As launch()'s cluster: no clusters, and the kernel may start before the stream's kernel before
+// it has ended (it waits for that end itself, before it reads what that kernel writes or writes
+// what it reads).
+constexpr int kAfterStart = 0;
+
 // kernel<<<grid, block, smem, s>>>(args...) in clusters of `cluster` CTAs, with the launch's own status (an error that an
 // earlier call of the program left behind is not taken for it). The opt-in to more than 48 KB of
 // shared memory is per device and kept in *opted, a bit per device.
@@ -41,11 +46,16 @@ void launch(std::atomic<unsigned long long>* opted, void (*kernel)(P...), dim3 g
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    if (cluster == kAfterStart) {
+      attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr[0].val.programmaticStreamSerializationAllowed = 1;
+    } else {
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = cluster;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    }
     cfg.attrs = attr;
-    cfg.numAttrs = cluster > 1 ? 1 : 0;
+    cfg.numAttrs = cluster != 1 ? 1 : 0;
     e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
   }
   if (e != cudaSuccess) {
@@ -85,7 +95,7 @@ struct BlocksView {
 // route.cu
 size_t route_workspace_bytes(long long pairs, int experts);
 int launch_route(const DenseView& ids, int experts, int* expert_ptr, int* row_pair, int* pair_row,
-                 int* counts, int sms, cudaStream_t s);
+                 int* counts, cudaStream_t s);
 // routed_rows.cu
 int launch_dispatch(const RoutesView& r, const DenseView& x, const void* w, const DenseView& y,
                     cudaStream_t s);

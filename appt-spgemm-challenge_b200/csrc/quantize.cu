@@ -3,10 +3,14 @@
 //   scale = max(amax / 448, smallest normal float),   q = e4m3(value / scale)
 //
 // value is X, or silu(X[:, :n]) X[:, n:]; for dispatch, a token's row is quantised once and
-// written to each of its pairs' rows. 16 lanes hold a block, 8 neighbouring columns each; the
-// largest magnitude is a maximum of the bit patterns without sign, in which a NaN is above
-// infinity, so neither is lost. Bound by memory: the quotients are true divisions (a product with
-// the reciprocal rounds differently), some 10 instructions per element and still below the copy.
+// written to each of its pairs' rows. 8 lanes hold a block, 16 neighbouring columns each; the
+// largest magnitude is a maximum that keeps a NaN. The quotients are rounded as divisions are (a
+// product with the reciprocal would round differently), at three instructions each.
+//
+// Bound by memory, but only just: at 25 (gated) instructions per element the SMs issue 70 % of
+// what they can. Gated bf16 16384 x 2048: 33 us, 5.1 TB/s (16-bit access, plain divisions and
+// 64-bit index arithmetic: 74 us). Routed bf16 8192 x 4096 to 8 experts each: 66 us, 5.2 TB/s (84
+// us); the scales' 4-byte writes land in rows far apart.
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <cfloat>
@@ -18,122 +22,185 @@ namespace appt {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kBlocksPerCta = kThreads / 16;   // scale blocks that a CTA holds at a time
+constexpr int kPer = 16;                              // columns of a lane
+constexpr int kLanes = kScaleBlock / kPer;            // lanes of a block
+constexpr int kBlocksPerCta = kThreads / kLanes;
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int n, bool vec, float v[8]) {
-  if (vec && n >= 8) {
+// n of a lane's 16 values, zeros behind them; n is 16 or 0 where kVec.
+template <bool kVec, typename T>
+__device__ __forceinline__ void load16(const T* p, int n, float (&v)[kPer]) {
+  if constexpr (kVec) {
     constexpr int N = 16 / sizeof(T);
 #pragma unroll
-    for (int i = 0; i < 8; i += N) {
-      const Pack<T, N> x = *(const Pack<T, N>*)(p + i);
+    for (int i = 0; i < kPer; i += N) {
+      float f[N] = {};
+      if (n) ((const Pack<T, N>*)(p + i))->up(f);
 #pragma unroll
-      for (int k = 0; k < N; ++k) v[i + k] = Value<T>::up(x.v[k]);
+      for (int k = 0; k < N; ++k) v[i + k] = f[k];
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? Value<T>::up(p[i]) : 0.f;
+    for (int i = 0; i < kPer; ++i) v[i] = i < n ? Value<T>::up(p[i]) : 0.f;
   }
+}
+
+// x / s in fp32, rounded to nearest as a division is, for many x with one s: with y the rounded
+// reciprocal and q = x y, one step q + (x - q s) y corrects the last place (Markstein's method; the
+// remainder is exact in an fma). Holds while neither s, its reciprocal nor the remainder leaves the
+// normal range; other scales (and those that are no numbers) divide.
+struct Divisor {
+  float s, y;
+  __device__ __forceinline__ explicit Divisor(float scale) {
+    s = scale;
+    y = __frcp_rn(scale);
+  }
+  __device__ __forceinline__ bool holds() const { return s > 0x1p-60f && s < 0x1p60f; }
+  __device__ __forceinline__ float of(float x) const {
+    const float q = x * y;
+    return __fmaf_rn(__fmaf_rn(-q, s, x), y, q);
+  }
+};
+
+// g / (1 + exp(-g)). 2^x and the reciprocal are the hardware's (2 steps and 1); the argument's
+// rounding adds |g| 2^-24, which for g > 0 the 1 in the sum damps. Where exp(-g) passes 2^126 the
+// reciprocal is 0, as 1 / infinity is a little further on.
+__device__ __forceinline__ float silu(float g) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.44269504f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return g * r;
+}
+
+// max(|a|, |b|, c), a NaN where one is
+__device__ __forceinline__ float abs_max(float a, float b, float c) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(c));
+  return m;
 }
 
 struct Target {
   unsigned char* q;
-  long long ld;
   float* scale;
-  long long scale_ld;
-  long long rows, cols;
-  bool vec;             // rows of q start on 8 bytes
+  long long cols;
+  int ld, scale_ld, rows;
 };
 
-__device__ __forceinline__ void store8(const Target& o, long long row, long long col, int n,
-                                       uint2 q) {
-  unsigned char* p = o.q + row * o.ld + col;
-  if (o.vec && n >= 8) {
-    *(uint2*)p = q;
+template <bool kVec>
+__device__ __forceinline__ void store16(unsigned char* p, int n, const unsigned (&q)[4]) {
+  if constexpr (kVec) {
+    if (n) *(uint4*)p = make_uint4(q[0], q[1], q[2], q[3]);
   } else {
-    const unsigned long long both = (unsigned long long)q.y << 32 | q.x;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) p[i] = (unsigned char)(both >> (8 * i));
+    for (int i = 0; i < kPer; ++i)
+      if (i < n) p[i] = (unsigned char)(q[i / 4] >> (8 * (i % 4)));
   }
 }
 
-template <typename T, bool kGated, bool kRouted>
+__device__ __forceinline__ unsigned e4m3x2(float lo, float hi) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+
+// kVec: every row of X (its gate's half too) and of Q starts on 16 bytes, and the columns are a
+// multiple of 16. 2^groups_log2 groups of 8 lanes work on a row.
+template <typename T, bool kGated, bool kRouted, bool kVec>
 __global__ void __launch_bounds__(kThreads)
-    quantize_kernel(const T* __restrict__ x, long long ldx, bool xvec, long long rows,
+    quantize_kernel(const T* __restrict__ x, long long ldx, long long rows,
                     const int* __restrict__ rows_ptr, const int* __restrict__ pair_row, int top_k,
-                    Target o) {
-  const int sub = threadIdx.x & 15;
-  const long long blocks = (o.cols + kScaleBlock - 1) / kScaleBlock;
+                    int groups_log2, Target o) {
+  const int sub = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  const unsigned mine = 0xffu << (threadIdx.x & 24);   // the block's lanes
+  const int blocks = (int)((o.cols + kScaleBlock - 1) / kScaleBlock);
+  const int step = 1 << groups_log2, per_cta = kBlocksPerCta >> groups_log2;
   if (!kRouted && rows_ptr) {
     const long long r = *rows_ptr;
     rows = r < rows ? (r > 0 ? r : 0) : rows;
   }
-  const long long items = rows * blocks;   // (row, block), blocks of a row next to each other
-  const long long step = (long long)gridDim.x * kBlocksPerCta;
-  // whole warps run the loop: the two halves' items differ by one
-  for (long long i0 = (long long)blockIdx.x * kBlocksPerCta + (threadIdx.x >> 5) * 2; i0 < items;
-       i0 += step) {
-    const long long i = i0 + ((threadIdx.x >> 4) & 1);
-    const bool on = i < items;
-    const long long row = on ? i / blocks : 0, block = on ? i % blocks : 0;
-    const long long col = block * kScaleBlock + sub * 8;
-    const int n = on ? (int)(o.cols - col < 8 ? (o.cols > col ? o.cols - col : 0) : 8) : 0;
-    float v[8];
-    const T* p = x + row * ldx + col;
-    load8(p, n, xvec, v);
-    if (kGated) {
-      float u[8];
-      load8(p + o.cols, n, xvec && o.cols % (16 / (int)sizeof(T)) == 0, u);
+  for (long long row = (long long)blockIdx.x * per_cta + (group >> groups_log2); row < rows;
+       row += (long long)gridDim.x * per_cta) {
+    for (int block = group & (step - 1); block < blocks; block += step) {
+      const long long col = (long long)block * kScaleBlock + sub * kPer;
+      const int n = col < o.cols ? (o.cols - col < kPer ? (int)(o.cols - col) : kPer) : 0;
+      const T* p = x + row * ldx + col;
+      float v[kPer];
+      load16<kVec>(p, n, v);
+      if (kGated) {
+        float up[kPer];
+        load16<kVec>(p + o.cols, n, up);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = v[k] / (1.f + expf(-v[k])) * u[k];
-    }
-    unsigned top = 0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[k]) & 0x7fffffffu);
-#pragma unroll
-    for (int s = 8; s > 0; s >>= 1) top = max(top, __shfl_xor_sync(kFull, top, s));
-    float scale = __fdiv_rn(__uint_as_float(top), 448.f);
-    if (scale < FLT_MIN) scale = FLT_MIN;   // false for NaN
-    unsigned q[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      q[k] = __nv_cvt_float2_to_fp8x2(
-          make_float2(__fdiv_rn(v[2 * k], scale), __fdiv_rn(v[2 * k + 1], scale)), __NV_SATFINITE,
-          __NV_E4M3);
-    const uint2 out = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
-    if (kRouted) {
-      if (!on) continue;
-      for (int j = 0; j < top_k; ++j) {
-        const int r = pair_row[row * top_k + j];
-        if (r < 0 || r >= o.rows) continue;
-        store8(o, r, col, n, out);
-        if (sub == 0) o.scale[block * o.scale_ld + r] = scale;
+        for (int k = 0; k < kPer; ++k) v[k] = silu(v[k]) * up[k];
       }
-    } else if (on) {
-      store8(o, row, col, n, out);
-      if (sub == 0) o.scale[block * o.scale_ld + row] = scale;
+      float top = 0.f;
+#pragma unroll
+      for (int k = 0; k < kPer; k += 2) top = abs_max(v[k], v[k + 1], top);
+#pragma unroll
+      for (int s = kLanes / 2; s > 0; s >>= 1)
+        top = abs_max(__shfl_xor_sync(mine, top, s), 0.f, top);
+      float scale = __fdiv_rn(top, 448.f);
+      if (scale < FLT_MIN) scale = FLT_MIN;   // false for NaN
+      const Divisor div(scale);
+      unsigned q[4];
+      if (div.holds()) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          q[k] = e4m3x2(div.of(v[4 * k]), div.of(v[4 * k + 1])) |
+                 e4m3x2(div.of(v[4 * k + 2]), div.of(v[4 * k + 3])) << 16;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          q[k] = e4m3x2(__fdiv_rn(v[4 * k], scale), __fdiv_rn(v[4 * k + 1], scale)) |
+                 e4m3x2(__fdiv_rn(v[4 * k + 2], scale), __fdiv_rn(v[4 * k + 3], scale)) << 16;
+      }
+      float* ps = o.scale + (long long)block * o.scale_ld;
+      if (kRouted) {
+        const int* pr = pair_row + row * top_k;
+        unsigned char* pq = o.q + col;
+        for (int j0 = 0; j0 < top_k; j0 += 4) {
+          int r[4];   // on their way together
+#pragma unroll
+          for (int j = 0; j < 4; ++j) r[j] = j0 + j < top_k ? pr[j0 + j] : -1;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if ((unsigned)r[j] >= (unsigned)o.rows) continue;
+            store16<kVec>(pq + (long long)r[j] * o.ld, n, q);
+            if (sub == 0) ps[r[j]] = scale;
+          }
+        }
+      } else {
+        store16<kVec>(o.q + row * o.ld + col, n, q);
+        if (sub == 0) ps[row] = scale;
+      }
     }
   }
+}
+
+template <typename T, bool kVec>
+void quantize(const DenseView& x, bool gated, const int* rows_ptr, const RoutesView* routes,
+              const Target& o, cudaStream_t s) {
+  const long long blocks = (o.cols + kScaleBlock - 1) / kScaleBlock;
+  int groups = 0;   // no more than a row has blocks
+  while (2 << groups <= kBlocksPerCta && 2 << groups <= blocks) ++groups;
+  const int per_cta = kBlocksPerCta >> groups;
+  const long long ctas = (x.rows + per_cta - 1) / per_cta;
+  const dim3 grid((unsigned)(ctas < (1 << 20) ? ctas : 1 << 20));
+  const T* p = (const T*)x.data;
+  if (routes)
+    launch(nullptr, quantize_kernel<T, false, true, kVec>, grid, kThreads, 0, s, 1, p, x.ld, x.rows,
+           nullptr, routes->pair_row, routes->top_k, groups, o);
+  else if (gated)
+    launch(nullptr, quantize_kernel<T, true, false, kVec>, grid, kThreads, 0, s, 1, p, x.ld, x.rows,
+           rows_ptr, nullptr, 1, groups, o);
+  else
+    launch(nullptr, quantize_kernel<T, false, false, kVec>, grid, kThreads, 0, s, 1, p, x.ld,
+           x.rows, rows_ptr, nullptr, 1, groups, o);
 }
 
 template <typename T>
 void quantize(const DenseView& x, bool gated, const int* rows_ptr, const RoutesView* routes,
               const Target& o, cudaStream_t s) {
-  const bool xvec = (uintptr_t)x.data % 16 == 0 && x.ld * sizeof(T) % 16 == 0;
-  const long long items = x.rows * ((o.cols + kScaleBlock - 1) / kScaleBlock);
-  const long long ctas = (items + kBlocksPerCta - 1) / kBlocksPerCta;
-  const dim3 grid((unsigned)(ctas < (1 << 20) ? ctas : 1 << 20));
-  const T* p = (const T*)x.data;
-  if (routes)
-    launch(nullptr, quantize_kernel<T, false, true>, grid, kThreads, 0, s, 1, p, x.ld, xvec, x.rows,
-           nullptr, routes->pair_row, routes->top_k, o);
-  else if (gated)
-    launch(nullptr, quantize_kernel<T, true, false>, grid, kThreads, 0, s, 1, p, x.ld, xvec, x.rows,
-           rows_ptr, nullptr, 1, o);
-  else
-    launch(nullptr, quantize_kernel<T, false, false>, grid, kThreads, 0, s, 1, p, x.ld, xvec, x.rows,
-           rows_ptr, nullptr, 1, o);
+  const bool vec = (uintptr_t)x.data % 16 == 0 && x.ld * sizeof(T) % 16 == 0 &&
+                   (uintptr_t)o.q % 16 == 0 && o.ld % 16 == 0 && o.cols % kPer == 0;
+  if (vec) quantize<T, true>(x, gated, rows_ptr, routes, o, s);
+  else quantize<T, false>(x, gated, rows_ptr, routes, o, s);
 }
 
 }  // namespace
@@ -141,8 +208,8 @@ void quantize(const DenseView& x, bool gated, const int* rows_ptr, const RoutesV
 int launch_quantize(const DenseView& x, bool gated, const int* rows_ptr, const RoutesView* routes,
                     const ScaledView& q, cudaStream_t s) {
   if (x.rows == 0 || q.q.cols == 0 || q.q.rows == 0) return 0;
-  const Target o{(unsigned char*)q.q.data, q.q.ld, q.scale, q.scale_ld, q.q.rows, q.q.cols,
-                 (uintptr_t)q.q.data % 8 == 0 && q.q.ld % 8 == 0};
+  const Target o{(unsigned char*)q.q.data, q.scale, q.q.cols, (int)q.q.ld, (int)q.scale_ld,
+                 (int)q.q.rows};
   switch (x.type) {
     case kF32: quantize<float>(x, gated, rows_ptr, routes, o, s); break;
     case kF16: quantize<__half>(x, gated, rows_ptr, routes, o, s); break;

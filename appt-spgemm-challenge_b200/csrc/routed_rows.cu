@@ -17,11 +17,15 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// Pieces that a thread of dispatch has in flight: 64 bytes, or 8 single elements where rows do not
+// start and end on 16 bytes.
+__host__ __device__ constexpr int pieces_in_flight(int elements) { return elements > 1 ? 4 : 8; }
+
 // What the three kernels share: `lanes` (a multiple of 32) threads per token.
 struct Shape {
   const int* pair_row;
   int tokens, top_k;
-  long long pieces;     // pieces of N elements per row
+  int pieces;           // pieces of N elements per row
   int lanes;
 };
 
@@ -37,7 +41,7 @@ __device__ __forceinline__ Place place(const Shape& s) {
 }
 
 // Rows (-1: dropped or out of range) of up to 32 pairs of a token, one per lane.
-__device__ __forceinline__ int lane_row(const Shape& s, int token, int j0, long long rows) {
+__device__ __forceinline__ int lane_row(const Shape& s, int token, int j0, int rows) {
   const int j = j0 + (threadIdx.x & 31);
   const int r = j < s.top_k ? s.pair_row[(long long)token * s.top_k + j] : -1;
   return r >= 0 && r < rows ? r : -1;
@@ -50,15 +54,16 @@ __device__ __forceinline__ A lane_weight(const Shape& s, const A* w, int token, 
 
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads)
-    dispatch_kernel(Shape s, const T* __restrict__ x, long long ldx,
-                    const typename Value<T>::Acc* __restrict__ w, T* __restrict__ y, long long ldy,
-                    long long rows) {
+    dispatch_kernel(Shape s, const T* __restrict__ x, int ldx,
+                    const typename Value<T>::Acc* __restrict__ w, T* __restrict__ y, int ldy,
+                    int rows) {
   using A = typename Value<T>::Acc;
   using P = Pack<T, N>;
-  constexpr int U = 4;
+  constexpr int U = pieces_in_flight(N);
   const Place me = place(s);
   if (me.token < 0) return;   // whole warps
-  const P* px = (const P*)(x + me.token * ldx);
+  const P* px = (const P*)(x + (long long)me.token * ldx);
+  // (64-bit: past the last piece of a long row, 32 bits could wrap)
   for (long long base = (long long)blockIdx.y * s.lanes * U; base < s.pieces;
        base += (long long)gridDim.y * s.lanes * U) {
     P v[U];
@@ -74,15 +79,18 @@ __global__ void __launch_bounds__(kThreads)
         const int row = __shfl_sync(kFull, mine, j);
         const A wj = __shfl_sync(kFull, wmine, j);
         if (row < 0) continue;
-        P* py = (P*)(y + row * ldy);
+        P* py = (P*)(y + (long long)row * ldy);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const long long c = base + me.at + (long long)u * s.lanes;
           if (c >= s.pieces) continue;
           P o = v[u];
           if (w) {
+            A f[N];
+            v[u].up(f);
 #pragma unroll
-            for (int i = 0; i < N; ++i) o.v[i] = Value<T>::down(wj * Value<T>::up(v[u].v[i]));
+            for (int i = 0; i < N; ++i) f[i] *= wj;
+            o.down(f);
           }
           py[c] = o;
         }
@@ -93,15 +101,15 @@ __global__ void __launch_bounds__(kThreads)
 
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads)
-    combine_kernel(Shape s, const T* __restrict__ h, long long ldh, long long rows,
+    combine_kernel(Shape s, const T* __restrict__ h, int ldh, int rows,
                    const typename Value<T>::Acc* __restrict__ w, T* __restrict__ y,
-                   long long ldy) {
+                   int ldy) {
   using A = typename Value<T>::Acc;
   using P = Pack<T, N>;
   constexpr int J = 4;   // rows in flight
   const Place me = place(s);
   if (me.token < 0) return;
-  P* py = (P*)(y + me.token * ldy);
+  P* py = (P*)(y + (long long)me.token * ldy);
   for (long long base = (long long)blockIdx.y * s.lanes; base < s.pieces;
        base += (long long)gridDim.y * s.lanes) {
     const long long c = base + me.at;
@@ -119,22 +127,23 @@ __global__ void __launch_bounds__(kThreads)
         for (int u = 0; u < J; ++u) {
           row[u] = __shfl_sync(kFull, mine, (j + u) & 31);   // lanes past top_k hold -1
           wj[u] = __shfl_sync(kFull, wmine, (j + u) & 31);
-          if (row[u] >= 0 && c < s.pieces) v[u] = ((const P*)(h + row[u] * ldh))[c];
+          if (row[u] >= 0 && c < s.pieces) v[u] = ((const P*)(h + (long long)row[u] * ldh))[c];
         }
         if (c < s.pieces) {
 #pragma unroll
           for (int u = 0; u < J; ++u) {
             if (row[u] < 0) continue;
+            A f[N];
+            v[u].up(f);
 #pragma unroll
-            for (int i = 0; i < N; ++i) sum[i] += wj[u] * Value<T>::up(v[u].v[i]);
+            for (int i = 0; i < N; ++i) sum[i] += wj[u] * f[i];
           }
         }
       }
     }
     if (c < s.pieces) {
       P o;
-#pragma unroll
-      for (int i = 0; i < N; ++i) o.v[i] = Value<T>::down(sum[i]);
+      o.down(sum);
       py[c] = o;
     }
   }
@@ -145,10 +154,10 @@ __global__ void __launch_bounds__(kThreads)
 // pieces, over the lanes, over the warps).
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads)
-    combine_grad_kernel(Shape s, const T* __restrict__ dy, long long ldy, const T* __restrict__ h,
-                        long long ldh, long long rows,
+    combine_grad_kernel(Shape s, const T* __restrict__ dy, int ldy, const T* __restrict__ h,
+                        int ldh, int rows,
                         const typename Value<T>::Acc* __restrict__ w, T* __restrict__ dh,
-                        long long lddh, typename Value<T>::Acc* __restrict__ dw) {
+                        int lddh, typename Value<T>::Acc* __restrict__ dw) {
   using A = typename Value<T>::Acc;
   using P = Pack<T, N>;
   constexpr int J = 4;
@@ -171,24 +180,27 @@ __global__ void __launch_bounds__(kThreads)
     }
     if (me.token >= 0) {
       for (long long c = me.at; c < s.pieces; c += s.lanes) {
-        const P g = py[c];
+        A g[N];
+        py[c].up(g);
         P v[J];
 #pragma unroll
         for (int u = 0; u < J; ++u)
-          if (dw && row[u] >= 0) v[u] = ((const P*)(h + row[u] * ldh))[c];
+          if (dw && row[u] >= 0) v[u] = ((const P*)(h + (long long)row[u] * ldh))[c];
 #pragma unroll
         for (int u = 0; u < J; ++u) {
           if (row[u] < 0) continue;
+          A f[N];
           if (dw) {
+            v[u].up(f);
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-              dot[u] += Value<T>::up(g.v[i]) * Value<T>::up(v[u].v[i]);
+            for (int i = 0; i < N; ++i) dot[u] += g[i] * f[i];
           }
           if (dh) {
-            P o;
 #pragma unroll
-            for (int i = 0; i < N; ++i) o.v[i] = Value<T>::down(wj[u] * Value<T>::up(g.v[i]));
-            ((P*)(dh + row[u] * lddh))[c] = o;
+            for (int i = 0; i < N; ++i) f[i] = wj[u] * g[i];
+            P o;
+            o.down(f);
+            ((P*)(dh + (long long)row[u] * lddh))[c] = o;
           }
         }
       }
@@ -214,7 +226,7 @@ bool wide(const DenseView& m, int bytes) {
   return (uintptr_t)m.data % 16 == 0 && m.ld * bytes % 16 == 0;
 }
 
-Shape shape_for(const RoutesView& r, long long pieces) {
+Shape shape_for(const RoutesView& r, int pieces) {
   Shape s{r.pair_row, r.tokens, r.top_k, pieces, 32};
   while (s.lanes < kThreads && s.lanes < pieces) s.lanes *= 2;
   return s;
@@ -222,7 +234,7 @@ Shape shape_for(const RoutesView& r, long long pieces) {
 
 dim3 grid_for(const Shape& s, long long per_cta_pieces) {
   const int per = kThreads / s.lanes;
-  const long long y = (s.pieces + per_cta_pieces - 1) / per_cta_pieces;
+  const long long y = ((long long)s.pieces + per_cta_pieces - 1) / per_cta_pieces;
   return dim3((s.tokens + per - 1) / per, (unsigned)(y > 65535 ? 65535 : y));
 }
 
@@ -259,8 +271,8 @@ int launch_dispatch(const RoutesView& r, const DenseView& x, const void* w, cons
   by_type(x.type, x.cols, wide(x, b) && wide(y, b), [&](auto t, auto n) {
     using T = decltype(t);
     constexpr int N = decltype(n)::value;
-    const Shape sh = shape_for(r, x.cols / N);
-    launch(nullptr, dispatch_kernel<T, N>, grid_for(sh, sh.lanes * 4), kThreads, 0, s, 1, sh,
+    const Shape sh = shape_for(r, (int)(x.cols / N));
+    launch(nullptr, dispatch_kernel<T, N>, grid_for(sh, sh.lanes * pieces_in_flight(N)), kThreads, 0, s, 1, sh,
            (const T*)x.data, x.ld, (const typename Value<T>::Acc*)w, (T*)y.data, y.ld, y.rows);
   });
   return 1;
@@ -273,7 +285,7 @@ int launch_combine(const RoutesView& r, const DenseView& h, const void* w, const
   by_type(h.type, h.cols, wide(h, b) && wide(y, b), [&](auto t, auto n) {
     using T = decltype(t);
     constexpr int N = decltype(n)::value;
-    const Shape sh = shape_for(r, h.cols / N);
+    const Shape sh = shape_for(r, (int)(h.cols / N));
     launch(nullptr, combine_kernel<T, N>, grid_for(sh, sh.lanes), kThreads, 0, s, 1, sh,
            (const T*)h.data, h.ld, h.rows, (const typename Value<T>::Acc*)w, (T*)y.data, y.ld);
   });
@@ -289,7 +301,7 @@ int launch_combine_grad(const RoutesView& r, const DenseView& dy, const DenseVie
     using T = decltype(t);
     using A = typename Value<T>::Acc;
     constexpr int N = decltype(n)::value;
-    const Shape sh = shape_for(r, dy.cols / N);
+    const Shape sh = shape_for(r, (int)(dy.cols / N));
     const int per = kThreads / sh.lanes;
     launch(nullptr, combine_grad_kernel<T, N>, (r.tokens + per - 1) / per, kThreads, 0, s, 1, sh,
            (const T*)dy.data, dy.ld, h ? (const T*)h->data : nullptr, h ? h->ld : 0,

@@ -111,24 +111,24 @@ __device__ __forceinline__ void write_rows(const Params& p, char* piece, const f
   for (int c0 = 0; c0 < N; c0 += kCols) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      Pack<T, kPer> o;
+      float f[kPer];
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) o.v[i] = Value<T>::down(v[c0 + j * kPer + i]);
+      for (int i = 0; i < kPer; ++i) f[i] = v[c0 + j * kPer + i];
+      Pack<T, kPer> o;
+      o.down(f);
       *(Pack<T, kPer>*)(piece + lane * kOutRow + (j ^ (lane >> 1 & 3)) * 16) = o;
     }
     __syncwarp();
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int r = k * 8 + lane / 4, j = lane & 3, n = n0 + c0 + j * kPer;
-      const Pack<T, kPer> o = *(Pack<T, kPer>*)(piece + r * kOutRow + (j ^ (r >> 1 & 3)) * 16);
+      const T* from = (const T*)(piece + r * kOutRow + (j ^ (r >> 1 & 3)) * 16);
       T* y = (T*)p.y + (row0 + r) * p.ldy + n;
       if (row0 + r >= row_end || n >= p.n) continue;
       if (n + kPer <= p.n) {
-        *(Pack<T, kPer>*)y = o;
+        *(uint4*)y = *(const uint4*)from;
       } else {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-          if (n + i < p.n) y[i] = o.v[i];
+        for (int i = 0; n + i < p.n; ++i) y[i] = from[i];
       }
     }
     __syncwarp();

@@ -4,6 +4,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <type_traits>
 
 namespace appt {
 
@@ -28,10 +29,63 @@ template <> struct Value<__nv_bfloat16> {
   static __device__ __forceinline__ __nv_bfloat16 down(float x) { return __float2bfloat16_rn(x); }
 };
 
-// N consecutive elements, moved as one access.
+// N consecutive elements moved as one access: one element, or 16 bytes kept as words (arrays of
+// 16-bit elements would take a register each).
 template <typename T, int N>
-struct alignas(sizeof(T) * N) Pack {
-  T v[N];
+struct Pack {
+  using A = typename Value<T>::Acc;
+  static constexpr int kPerWord = 4 / sizeof(T);
+  uint4 w;
+  __device__ __forceinline__ void up(A (&v)[N]) const {
+    static_assert(sizeof(T) * N == 16, "");
+    const unsigned word[4] = {w.x, w.y, w.z, w.w};
+    if constexpr (sizeof(T) == 8) {
+      v[0] = __hiloint2double((int)w.y, (int)w.x);
+      v[1] = __hiloint2double((int)w.w, (int)w.z);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+          v[i] = __uint_as_float(word[i]);
+        } else if constexpr (std::is_same<T, __half>::value) {
+          const __half2_raw r{(unsigned short)word[i], (unsigned short)(word[i] >> 16)};
+          const float2 f = __half22float2(__half2(r));
+          v[2 * i] = f.x, v[2 * i + 1] = f.y;
+        } else {   // bf16 is the upper half of fp32
+          v[2 * i] = __uint_as_float(word[i] << 16);
+          v[2 * i + 1] = __uint_as_float(word[i] & 0xffff0000u);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void down(const A (&v)[N]) {
+    unsigned word[4];
+    if constexpr (sizeof(T) == 8) {
+      word[0] = (unsigned)__double2loint(v[0]), word[1] = (unsigned)__double2hiint(v[0]);
+      word[2] = (unsigned)__double2loint(v[1]), word[3] = (unsigned)__double2hiint(v[1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+          word[i] = __float_as_uint(v[i]);
+        } else if constexpr (std::is_same<T, __half>::value) {
+          const __half2_raw r(__floats2half2_rn(v[2 * i], v[2 * i + 1]));
+          word[i] = r.x | (unsigned)r.y << 16;
+        } else {
+          const __nv_bfloat162_raw r(__floats2bfloat162_rn(v[2 * i], v[2 * i + 1]));
+          word[i] = r.x | (unsigned)r.y << 16;
+        }
+      }
+    }
+    w = make_uint4(word[0], word[1], word[2], word[3]);
+  }
+};
+template <typename T>
+struct Pack<T, 1> {
+  using A = typename Value<T>::Acc;
+  T w;
+  __device__ __forceinline__ void up(A (&v)[1]) const { v[0] = Value<T>::up(w); }
+  __device__ __forceinline__ void down(const A (&v)[1]) { w = Value<T>::down(v[0]); }
 };
 
 }  // namespace appt

@@ -323,7 +323,8 @@ int appt_comm_spgemm(appt_comm *comm, const appt_csr *A_block, const appt_csr *B
 
 typedef struct appt_dense { /* row-major dense matrix in device memory */
   int64_t rows, cols;
-  int64_t ld;       /* elements from one row to the next, >= cols (ignored with fewer than 2 rows) */
+  int64_t ld;       /* elements from one row to the next, cols <= ld < 2^31 - 1 (ignored with
+                       fewer than 2 rows) */
   void *data;
   int32_t type;     /* APPT_F64 .. APPT_I64 */
   int32_t reserved; /* 0 */
@@ -340,7 +341,7 @@ typedef struct appt_routes { /* where each pair went, as appt_route fills it */
 typedef struct appt_scaled { /* values in 8 bits with one scale per row and block of 128 columns */
   appt_dense q;     /* APPT_E4M3 */
   float *scale;     /* scale[b * scale_ld + r] belongs to row r, columns 128 b .. 128 b + 127 */
-  int64_t scale_ld; /* >= q.rows */
+  int64_t scale_ld; /* q.rows <= scale_ld < 2^31 - 1 (ignored with one block) */
 } appt_scaled;
 
 typedef struct appt_blocks { /* `groups` matrices in 8 bits, one scale per block of 128 x 128 */

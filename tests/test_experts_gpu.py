@@ -107,7 +107,8 @@ def check_route(ids, experts, ptr, row_pair, pair_row):
     (33, 3, 1024, "any"), (32, 8, 64, "any"), (511, 8, 64, "same"), (512, 8, 64, "wild"),
     (513, 8, 64, "skew"), (1000, 40, 100, "wild"), (4097, 1, 1023, "any"), (20000, 3, 1, "wild"),
     (5000, 7, 512, "skew"), (70001, 8, 256, "wild"), (131073, 8, 333, "skew"),
-    (66000, 8, 1024, "none"), (66000, 8, 1024, "same")])
+    (66000, 8, 1024, "none"), (66000, 8, 1024, "same"), (3000, 4, 1024, "wild"),
+    (4000, 8, 100, "skew"), (4096, 8, 33, "any"), (32769, 1, 64, "any")])
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
 def test_route(tokens, top_k, experts, kind, dtype):
     ids = ids_for(gen(tokens + top_k), tokens, top_k, experts, kind).to(dtype)
@@ -777,13 +778,11 @@ def test_refusals_that_need_a_device():
     pinned = torch.zeros(4, 8).pin_memory()
     with pytest.raises(ap.ApptError, match="not memory of device"):
         ex.Dispatch(r, ex.Dense(pinned.data_ptr(), (4, 8), "f32"), y).run(stream())
-    far = ex.Dispatch(r, x, y)
-    far._device = 63
-    with pytest.raises(ap.ApptError, match="device ordinal"):
-        far.run(stream())
-    far._device = -1
-    with pytest.raises(ap.ApptError, match="device ordinal"):
-        far.run(stream())
+    for device in (63, -1):
+        far = [ex.Dense(t.data_ptr(), tuple(t.shape), "f32", device=device) for t in (x, y)]
+        rows = ex.Dense(r.pair_row.data_ptr(), (8,), "i32", device=device)
+        with pytest.raises(ap.ApptError, match="device ordinal"):
+            ex.Dispatch(ex.Routes(4, 2, rows), *far).run(stream())
     before = ap.kernel_launches()
     ex.Dispatch(r, x, y).run(stream())
     assert ap.kernel_launches() == before + 1
