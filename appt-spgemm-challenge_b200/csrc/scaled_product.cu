@@ -44,7 +44,7 @@ constexpr int kScaleStages = 8;
 constexpr int kMaxStages = 10;
 constexpr int kMaxBuffers = 4;
 constexpr int kSharedMax = 227 * 1024;
-constexpr int kOutRow = 64, kOutWarp = 32 * kOutRow;   // a warp's piece of Y on its way out
+constexpr int kOutBox = 32 * 128;
 
 struct Params {
   const float* sa;
@@ -77,14 +77,16 @@ struct Shape {
   static constexpr int kNTile = kSwap ? kLanes : kCols;        // columns of Y per tile
   static constexpr int kScaleFloats = kSwap ? kCols + 4 : 0;   // the rows', then the weights'
   static constexpr int kBuffers = 512 / kCols < kMaxBuffers ? 512 / kCols : kMaxBuffers;
-  // 128 sums a thread: the adding warps take registers of the other four. 128 x 56 + 256 x 224 =
+  // 128 sums a thread: the adding warps take registers of the other four. 128 x 104 + 256 x 200 =
   // 64,512, the 384 x 168 that the launch holds.
   static constexpr bool kMoveRegs = kCols == 256;
   static constexpr int kTmemColumns = kBuffers * kCols < 32 ? 32 : kBuffers * kCols;
-  static constexpr int kGroups = 2;               // adding warpgroups
+  static constexpr int kGroups = 2;                            // adding warpgroups
   static constexpr int kThreads = 128 + 128 * kGroups;
   static constexpr int kPart = kCols / kGroups;                // columns of a warpgroup
-  static constexpr int kOutBytes = kSwap ? 0 : 4 * kGroups * kOutWarp;
+  // Y on its way out: a warp's boxes of 32 rows x 128 bytes, enough for its 16-bit values
+  static constexpr int kOutBoxes = kPart / 64;
+  static constexpr int kOutBytes = kSwap ? 0 : 4 * kGroups * kOutBoxes * kOutBox;
   static constexpr int kFixedBytes = kOutBytes + (int)sizeof(Groups) + (int)sizeof(Barriers) + 64 +
                                      kScaleStages * kScaleFloats * 4 + 1024;
   static constexpr int kStages = (kSharedMax - kFixedBytes) / kStageBytes < kMaxStages
@@ -99,39 +101,53 @@ __device__ __forceinline__ void store_one(const Params& p, long long at, float v
   else ((__nv_bfloat16*)p.y)[at] = __float2bfloat16_rn(v);
 }
 
-// A warp's 32 rows x N columns of Y, a row per thread, by way of shared memory: 64 bytes of each
-// row at a time, so that a store writes 8 rows' whole 64 bytes instead of 16 bytes of 32 rows.
-// Pieces of 16 bytes change places by the row, which spreads both accesses over all banks.
-template <typename T, int N>
-__device__ __forceinline__ void write_rows(const Params& p, char* piece, const float* v, int row0,
-                                           int row_end, int n0) {
-  constexpr int kPer = 16 / sizeof(T), kCols = kOutRow / sizeof(T);
+// A warp's 32 rows x N columns of Y, a row per thread, through boxes in shared memory that TMA
+// copies while the warp goes on with its next tile. The 16-byte pieces of a row change places by
+// the row (the 128-byte swizzle), which spreads the threads over the banks. Stores from registers
+// are 16 bytes of 32 rows at a time and took 4,500 cycles a tile, this takes a quarter.
+// A group's last rows, and rows that TMA cannot address, are stored from the boxes instead.
+template <typename T, int N, int kBoxes>
+__device__ __forceinline__ void write_rows(const Params& p, const CUtensorMap* map, char* boxes,
+                                           const uint64_t* v, int row, int rows, int n) {
+  constexpr int kPer = 16 / sizeof(T), kCols = 128 / sizeof(T), kPieces = 8 * kBoxes;
   const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int c0 = 0; c0 < N; c0 += kCols) {
+  for (int c0 = 0; c0 < N; c0 += kBoxes * kCols) {   // once, or twice for 32 bits
+    bulk_wait_read();                                // the copies before these (the issuer's)
+    __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int c = c0; c < c0 + kBoxes * kCols; c += kPer) {
+      char* box = boxes + (c - c0) / kCols * kOutBox;
       float f[kPer];
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) f[i] = v[c0 + j * kPer + i];
+      for (int i = 0; i < kPer; i += 2) untwo(v[(c + i) / 2], f[i], f[i + 1]);
       Pack<T, kPer> o;
       o.down(f);
-      *(Pack<T, kPer>*)(piece + lane * kOutRow + (j ^ (lane >> 1 & 3)) * 16) = o;
+      *(Pack<T, kPer>*)(box + lane * 128 + ((c % kCols) / kPer ^ (lane & 7)) * 16) = o;
     }
-    __syncwarp();
+    if (p.vec && rows >= 32) {
+      bulk_fence();
+      __syncwarp();
+      if (lane == 0) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int r = k * 8 + lane / 4, j = lane & 3, n = n0 + c0 + j * kPer;
-      const T* from = (const T*)(piece + r * kOutRow + (j ^ (r >> 1 & 3)) * 16);
-      T* y = (T*)p.y + (row0 + r) * p.ldy + n;
-      if (row0 + r >= row_end || n >= p.n) continue;
-      if (n + kPer <= p.n) {
-        *(uint4*)y = *(const uint4*)from;
-      } else {
-        for (int i = 0; n + i < p.n; ++i) y[i] = from[i];
+        for (int b = 0; b < kBoxes; ++b)
+          tma_store_2d(map, n + c0 + b * kCols, row, smem_u32(boxes + b * kOutBox));
+        bulk_commit();
+      }
+    } else {
+      __syncwarp();
+      const int j = lane % kPieces, c = c0 + j * kPer, cols = p.n - n - c;
+      for (int r = lane / kPieces; r < min(rows, 32); r += 32 / kPieces) {
+        const T* from =
+            (const T*)(boxes + j / 8 * kOutBox + r * 128 + ((j % 8) ^ (r & 7)) * 16);
+        T* y = (T*)p.y + (row + r) * p.ldy + n + c;
+        if (p.vec && cols >= kPer) {
+          *(uint4*)y = *(const uint4*)from;
+        } else {
+          for (int i = 0; i < min(cols, kPer); ++i) y[i] = from[i];
+        }
       }
     }
-    __syncwarp();
   }
 }
 
@@ -173,27 +189,44 @@ struct Tile {
   int group, row, row_end, n;    // first row, end of the group's rows, first column of Y
 };
 
+// A CTA's tiles, in order: index i, i + step, ... in rows of n_tiles tiles.
 template <int kRowTile, int kNTile>
-__device__ __forceinline__ Tile tile_at(const Params& p, const Groups* t, int i, int n_tiles) {
-  const int rt = i / n_tiles;
-  int lo = 0, hi = p.groups - 1;   // the last group whose first tile is <= rt
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (t->tile[mid] <= rt) lo = mid; else hi = mid - 1;
+struct Tiles {
+  const Groups* t;
+  int tiles, n_tiles, i, step, step_rows, step_cols, row, col, group;
+  __device__ __forceinline__ Tiles(const Groups* groups, int tiles_, int n_tiles_, int first,
+                                   int step_)
+      : t(groups), tiles(tiles_), n_tiles(n_tiles_), i(first), step(step_) {
+    step_rows = step / n_tiles;
+    step_cols = step - step_rows * n_tiles;
+    row = i / n_tiles;
+    col = i - row * n_tiles;
+    group = 0;
   }
-  return Tile{lo, t->row[lo] + (rt - t->tile[lo]) * kRowTile, t->row[lo + 1],
-              (i - rt * n_tiles) * kNTile};
-}
+  __device__ __forceinline__ bool more() const { return i < tiles; }
+  __device__ __forceinline__ Tile at() {
+    while (t->tile[group + 1] <= row) ++group;   // ends: row is below the last entry
+    return Tile{group, t->row[group] + (row - t->tile[group]) * kRowTile, t->row[group + 1],
+                col * kNTile};
+  }
+  __device__ __forceinline__ void next() {
+    i += step;
+    row += step_rows;
+    col += step_cols;
+    if (col >= n_tiles) col -= n_tiles, ++row;
+  }
+};
 
 template <bool kSwap, int kCols>
 __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_a,
-                   const __grid_constant__ CUtensorMap map_w, const Params p, int splits) {
+                   const __grid_constant__ CUtensorMap map_w,
+                   const __grid_constant__ CUtensorMap map_y, const Params p, int splits) {
   using S = Shape<kSwap, kCols>;
   constexpr int kPart = S::kPart;             // columns of a warpgroup
   extern __shared__ char raw[];
   char* base = (char*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
-  char* out = base + S::kStages * S::kStageBytes;
+  char* out = base + S::kStages * S::kStageBytes;   // on 1024 bytes, as the swizzle wants it
   Groups* groups = (Groups*)(out + S::kOutBytes);
   float* scales = (float*)(groups + 1);
   Barriers* bars = (Barriers*)(((uintptr_t)(scales + kScaleStages * S::kScaleFloats) + 7) &
@@ -231,18 +264,19 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
   const int tiles = groups->tile[p.groups] * n_tiles;   // below 2^31: checked by the host
   const int rank = splits > 1 ? (int)cluster_rank() : 0;
   const int first = blockIdx.x / splits, step = gridDim.x / splits;
+  Tiles<S::kRowTile, S::kNTile> order(groups, tiles, n_tiles, first, step);
   const int kb0 = (int)((long long)p.k_blocks * rank / splits);
   const int kb1 = (int)((long long)p.k_blocks * (rank + 1) / splits);
 
   if (warp < 4) {
-    if (S::kMoveRegs) regs_fewer<56>();
+    if (S::kMoveRegs) regs_fewer<104>();
     if (warp == 0) {
       // ---- tiles by TMA
       int it = 0, st = 0;
       uint32_t phase = 1;
       bool ok = true;
-      for (int i = first; ok && i < tiles; i += step) {
-        const Tile t = tile_at<S::kRowTile, S::kNTile>(p, groups, i, n_tiles);
+      for (; ok && order.more(); order.next()) {
+        const Tile t = order.at();
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           ok = mbar_wait(smem_u32(&bars->empty[st]), phase, gave_up);
           if (!ok) break;
@@ -258,15 +292,14 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
       }
       if (!ok)   // let the loads in flight land before the CTA ends
         for (int j = max(0, it - S::kStages); j < it; ++j)
-          for (int n = 0; n < kWaitTries; ++n)
-            if (mbar_try(smem_u32(&bars->full[j % S::kStages]), j / S::kStages & 1)) break;
+          mbar_drain(smem_u32(&bars->full[j % S::kStages]), j / S::kStages & 1);
     } else if (warp == 1) {
       // ---- products
       constexpr uint32_t idesc = instr_desc(kLanes, kCols);
       int st = 0, b = 0;
       uint32_t phase = 0, bphase = 1;
       bool ok = true;
-      for (int i = first; ok && i < tiles; i += step) {
+      for (; ok && order.more(); order.next()) {
         for (int kb = kb0; kb < kb1; ++kb) {
           ok = mbar_wait(smem_u32(&bars->full[st]), phase, gave_up) &&
                mbar_wait(smem_u32(&bars->tempty[b]), bphase, gave_up);
@@ -289,15 +322,14 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
       // products (and their arrivals) in flight end before the CTA does
       if (elect_one()) mma_commit(smem_u32(&bars->drain));
       __syncwarp();
-      for (int n = 0; n < kWaitTries; ++n)
-        if (mbar_try(smem_u32(&bars->drain), 0)) break;
+      mbar_drain(smem_u32(&bars->drain), 0);
     } else if (kSwap) {
       // ---- scales
       const int me = threadIdx.x - 64;
       int it = 0;
       bool ok = true;
-      for (int i = first; ok && i < tiles; i += step) {
-        const Tile t = tile_at<S::kRowTile, S::kNTile>(p, groups, i, n_tiles);
+      for (; ok && order.more(); order.next()) {
+        const Tile t = order.at();
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int st = it % kScaleStages;
           ok = mbar_wait(smem_u32(&bars->sempty[st]), (it / kScaleStages & 1) ^ 1, gave_up);
@@ -319,7 +351,7 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
     __syncwarp();
   } else {
     // ---- scaling, adding, writing
-    if (S::kMoveRegs) regs_more<224>();
+    if (S::kMoveRegs) regs_more<200>();
     const int wg = (warp - 4) / 4, quarter = warp & 3;
     const int who = quarter * 32 + lane;         // lane of the tile
     const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16) + wg * kPart;
@@ -332,7 +364,7 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
     auto buffer_read = [&](int n) {
       fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&bars->tempty[n % S::kBuffers]));
+      if (lane == 0) mbar_arrive_relaxed(smem_u32(&bars->tempty[n % S::kBuffers]));
     };
     auto clear = [&] {
 #pragma unroll
@@ -350,88 +382,55 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
         a0 = pa[0], w0 = pw[0];
         a1 = pa[second * p.sa_ld], w1 = pw[second];
       };
-      // Adds one partial tile, 16 columns at a time: the next 16 are on their way while these are
-      // added, across the end of the tile too, whose barrier is asked for 16 columns early.
-      constexpr int kChunk = 16, kChunks = kPart / kChunk;
-      static_assert(kChunks % 2 == 0, "a tile begins in the first array");
-      uint32_t part[2][kChunk];
-      auto start = [&] {
-        ok = mbar_wait(full_bar(it), full_phase(it), gave_up);
-        fence_after();
-        if (ok) tmem_load(part[0], buffer(it));
-      };
+      // Adds one partial tile, kChunk columns at a time, and hands its buffer back as soon as the
+      // last of them is in registers.
+      constexpr int kChunk = 16;
       // (no copy from one pair of scales to the other: it would wait for a load in flight)
       auto block = [&](float& a, float& w, int kb) {
+        ok = mbar_wait(full_bar(it), full_phase(it), gave_up);
+        if (!ok) return;
+        fence_after();
         const uint64_t scale = two(a * w, a * w);
         const int then = min(kb + 2, p.k_blocks - 1);
-        a = pa[then * p.sa_ld], w = pw[then];
-        const bool more = kb + 1 < p.k_blocks;
-        bool ready = false;
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          uint32_t(&now)[kChunk] = part[c & 1];
-          uint32_t(&next)[kChunk] = part[c & 1 ^ 1];
+        for (int c = 0; c < kPart; c += kChunk) {
+          uint32_t now[kChunk];
+          tmem_load(now, buffer(it) + c);
+          if (c == 0) a = pa[then * p.sa_ld], w = pw[then];
           tmem_wait(now);
-          if (c + 1 < kChunks) {
-            tmem_load(next, buffer(it) + (c + 1) * kChunk);
-          } else {
-            buffer_read(it);
-            if (more) {
-              if (!__all_sync(kFull, ready))
-                ok = mbar_wait(full_bar(it + 1), full_phase(it + 1), gave_up);
-              fence_after();
-              if (ok) tmem_load(next, buffer(it + 1));
-            }
-          }
-          if (c + 2 == kChunks && more) ready = mbar_try(full_bar(it + 1), full_phase(it + 1));
+          if (c + kChunk == kPart) buffer_read(it);
 #pragma unroll
           for (int j = 0; j < kChunk; j += 2)
-            pairs[(c * kChunk + j) / 2] =
-                fma_two(now[j], now[j + 1], scale, pairs[(c * kChunk + j) / 2]);
+            pairs[(c + j) / 2] = fma_two(now[j], now[j + 1], scale, pairs[(c + j) / 2]);
         }
         ++it;
       };
       Tile t = {};
-      if (first < tiles) {
-        t = tile_at<S::kRowTile, S::kNTile>(p, groups, first, n_tiles);
-        begin(t);
-      }
-      for (int i = first; i < tiles; i += step) {
+      if (order.more()) begin(t = order.at());
+      while (order.more()) {
         clear();
-        start();
         for (int kb = 0; ok && kb < p.k_blocks; kb += 2) {
           block(a0, w0, kb);
           if (ok && kb + 1 < p.k_blocks) block(a1, w1, kb + 1);
         }
         if (!ok) break;
         const Tile done = t;
-        if (i + step < tiles) {
-          t = tile_at<S::kRowTile, S::kNTile>(p, groups, i + step, n_tiles);
-          begin(t);
-        }
-        float sum[kPart];
-#pragma unroll
-        for (int c = 0; c < kPart; c += 2) untwo(pairs[c / 2], sum[c], sum[c + 1]);
-        char* piece = out + (warp - 4) * kOutWarp;
-        const int row0 = done.row + quarter * 32, n0 = done.n + wg * kPart;
-        if (!p.vec) {
-          if (row0 + lane < done.row_end) {
-            const long long at = (row0 + lane) * p.ldy + n0;
-#pragma unroll
-            for (int c = 0; c < kPart; ++c)
-              if (n0 + c < p.n) store_one(p, at + c, sum[c]);
-          }
-        } else if (p.type == kF32) {
-          write_rows<float, kPart>(p, piece, sum, row0, done.row_end, n0);
-        } else if (p.type == kF16) {
-          write_rows<__half, kPart>(p, piece, sum, row0, done.row_end, n0);
-        } else {
-          write_rows<__nv_bfloat16, kPart>(p, piece, sum, row0, done.row_end, n0);
-        }
+        order.next();
+        if (order.more()) begin(t = order.at());
+        const int row = done.row + quarter * 32, rows = done.row_end - row, n = done.n + wg * kPart;
+        if (rows <= 0 || n >= p.n) continue;
+        char* boxes = out + (warp - 4) * S::kOutBoxes * kOutBox;
+        if (p.type == kF32)
+          write_rows<float, kPart, S::kOutBoxes>(p, &map_y, boxes, pairs, row, rows, n);
+        else if (p.type == kF16)
+          write_rows<__half, kPart, S::kOutBoxes>(p, &map_y, boxes, pairs, row, rows, n);
+        else
+          write_rows<__nv_bfloat16, kPart, S::kOutBoxes>(p, &map_y, boxes, pairs, row, rows, n);
       }
+      bulk_wait();
     } else {
-      for (int i = first; i < tiles; i += step) {
-        const Tile t = tile_at<S::kRowTile, S::kNTile>(p, groups, i, n_tiles);
+      for (; order.more(); order.next()) {
+        const Tile t = order.at();
         clear();
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int st = it % kScaleStages;
@@ -479,7 +478,7 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
       // one tile per cluster: every CTA adds its share of the columns over all ranks
       cluster_sync();
       if (first < tiles && warp >= 4) {
-        const Tile t = tile_at<S::kRowTile, S::kNTile>(p, groups, first, n_tiles);
+        const Tile t = Tiles<S::kRowTile, S::kNTile>(groups, tiles, n_tiles, first, step).at();
         const int who = threadIdx.x & (kLanes - 1), wg = (warp - 4) / 4;
         for (int c = rank + splits * wg; c < kCols; c += 2 * splits) {
           const int r = t.row + c;
@@ -520,14 +519,18 @@ EncodeTiled encode_tiled() {
   return (EncodeTiled)fn;
 }
 
-// Boxes of `box` rows x 128 bytes, swizzled; columns and rows outside the matrix read as zeros.
+// Boxes of `box` rows x 128 bytes, swizzled, of elements of `bytes`; columns and rows outside the
+// matrix read as zeros. Strides are in bytes.
 CUtensorMap map_of(const void* data, long long cols, long long rows, long long ld,
-                   long long groups, long long group_stride, int box, int dims) {
+                   long long groups, long long group_stride, int box, int dims, int bytes = 1) {
   CUtensorMap m;
   const cuuint64_t size[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)groups};
   const cuuint64_t stride[2] = {(cuuint64_t)ld, (cuuint64_t)group_stride};
-  const cuuint32_t boxes[3] = {kScaleBlock, (cuuint32_t)box, 1}, ones[3] = {1, 1, 1};
-  if (encode_tiled()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, dims, const_cast<void*>(data), size, stride,
+  const cuuint32_t boxes[3] = {128u / bytes, (cuuint32_t)box, 1}, ones[3] = {1, 1, 1};
+  const CUtensorMapDataType type = bytes == 4   ? CU_TENSOR_MAP_DATA_TYPE_UINT32
+                                   : bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
+                                                : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  if (encode_tiled()(&m, type, dims, const_cast<void*>(data), size, stride,
                      boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
@@ -544,6 +547,11 @@ void product(const ScaledView& a, const BlocksView& w, const Params& p, int sms,
   const CUtensorMap ma = map_of(a.q.data, a.q.cols, a.q.rows, a.q.ld, 1, 0, S::kRowTile, 2);
   const CUtensorMap mw =
       map_of(w.data, w.cols, w.rows, w.ld, w.groups, w.group_stride, S::kNTile, 3);
+  CUtensorMap my = ma;   // (of Y only where its rows allow one)
+  if (!kSwap && p.vec) {
+    const int b = p.type == kF32 ? 4 : 2;
+    my = map_of(p.y, p.n, p.rows, p.ldy * b, 1, 0, 32, 2, b);
+  }
   // the most tiles that the groups' sizes allow
   const long long n_tiles = (p.n + S::kNTile - 1) / S::kNTile;
   const long long row_tiles =
@@ -555,7 +563,7 @@ void product(const ScaledView& a, const BlocksView& w, const Params& p, int sms,
     while (splits < 8 && tiles * splits * 2 <= sms && splits * 2 <= p.k_blocks) splits *= 2;
   const long long ctas = splits > 1 ? tiles * splits : tiles < sms ? tiles : sms;
   launch(&opted, product_kernel<kSwap, kCols>, dim3((unsigned)ctas), dim3(S::kThreads), S::kBytes, s,
-         splits, ma, mw, p, splits);
+         splits, ma, mw, my, p, splits);
 }
 
 }  // namespace

@@ -25,6 +25,11 @@ __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
                : "memory");
 }
+// An arrival that orders reads of tensor memory alone, which are done by then (tmem_wait,
+// fence_before): one that releases would first wait for the thread's loads from global memory.
+__device__ __forceinline__ void mbar_arrive_relaxed(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
@@ -36,19 +41,33 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return done != 0;
 }
-// Waits are bounded: a wait that runs out, or that sees that another one did, gives up. A try
-// suspends the thread for up to about a microsecond, so the bound is some seconds. Whole warps
-// wait, and the vote keeps them together: a wait by a single thread of a warp, in a branch that
-// the others skip, measured 205 cycles on a barrier that is ready, a whole warp's 70.
-constexpr int kWaitTries = 1 << 22;
+
+// Waits are bounded: a wait of two seconds, or one that sees that another gave up, gives up. Whole
+// warps wait, and the vote keeps them together: a wait by a single thread of a warp, in a branch
+// that the others skip, measured 205 cycles on a barrier that is ready, a whole warp's 70.
+constexpr int kWaitTries = 1 << 26;
+constexpr unsigned long long kWaitNs = 2000000000ull;
+__device__ __forceinline__ unsigned long long now_ns() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
   if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
+  const unsigned long long began = now_ns();
   for (int i = 0; i < kWaitTries; ++i) {
     if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
-    if ((i & 255) == 255 && __any_sync(0xffffffffu, *gave_up)) return false;
+    if ((i & 63) == 63 &&
+        __any_sync(0xffffffffu, *gave_up != 0 || now_ns() - began > kWaitNs)) break;
   }
   *gave_up = 1;
   return false;
+}
+// What is still in flight when a kernel gives up, or ends: the same without the flag.
+__device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
+  const unsigned long long began = now_ns();
+  for (int i = 0; i < kWaitTries && !mbar_try(bar, parity); ++i)
+    if ((i & 63) == 63 && now_ns() - began > kWaitNs) break;
 }
 // One thread of a converged warp; the compiler knows that it is one (a product issued under a
 // comparison of lanes took 50 cycles, under this 8).
@@ -59,7 +78,6 @@ __device__ __forceinline__ bool elect_one() {
   return one != 0;
 }
 
-// ------------------------------------------------------------------------------------------- TMA
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* map, int x, int y,
                                             uint32_t bar) {
   asm volatile(
@@ -75,6 +93,27 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* map, int x
       "{%2, %3, %4}], [%5];" ::"r"(dst),
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
+}
+// A box from shared memory; the part of it outside the tensor is not written. Whoever wrote the
+// shared memory fences after that, and one thread issues, commits, and waits before anyone writes
+// there again or the CTA ends.
+__device__ __forceinline__ void tma_store_2d(const void* map, int x, int y, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                   map),
+               "r"(x), "r"(y), "r"(src)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_fence() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+__device__ __forceinline__ void bulk_commit() {
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+__device__ __forceinline__ void bulk_wait() {
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 __device__ __forceinline__ void tma_prefetch_map(const void* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
@@ -94,7 +133,6 @@ __device__ __forceinline__ void cp_async_wait_all() {
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// --------------------------------------------------------------------------------- tensor memory
 __device__ __forceinline__ void tmem_alloc(uint32_t smem_slot, uint32_t columns) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_slot),
                "r"(columns)
