@@ -77,7 +77,7 @@ struct Shape {
   static constexpr int kNTile = kSwap ? kLanes : kCols;        // columns of Y per tile
   static constexpr int kScaleFloats = kSwap ? kCols + 4 : 0;   // the rows', then the weights'
   static constexpr int kBuffers = 512 / kCols < kMaxBuffers ? 512 / kCols : kMaxBuffers;
-  // 128 sums a thread: the adding warps take registers of the other four. 128 x 104 + 256 x 200 =
+  // 128 sums a thread: the adding warps take registers of the other four. 128 x 72 + 256 x 216 =
   // 64,512, the 384 x 168 that the launch holds.
   static constexpr bool kMoveRegs = kCols == 256;
   static constexpr int kTmemColumns = kBuffers * kCols < 32 ? 32 : kBuffers * kCols;
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
   const int kb1 = (int)((long long)p.k_blocks * (rank + 1) / splits);
 
   if (warp < 4) {
-    if (S::kMoveRegs) regs_fewer<104>();
+    if (S::kMoveRegs) regs_fewer<72>();
     if (warp == 0) {
       // ---- tiles by TMA
       int it = 0, st = 0;
@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
     __syncwarp();
   } else {
     // ---- scaling, adding, writing
-    if (S::kMoveRegs) regs_more<200>();
+    if (S::kMoveRegs) regs_more<216>();
     const int wg = (warp - 4) / 4, quarter = warp & 3;
     const int who = quarter * 32 + lane;         // lane of the tile
     const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16) + wg * kPart;
@@ -538,6 +538,12 @@ CUtensorMap map_of(const void* data, long long cols, long long rows, long long l
   return m;
 }
 
+// The most tiles along the rows that groups of any sizes can have (one group's size is known).
+long long row_tiles_for(long long rows, long long groups, int tile) {
+  if (groups == 1) return (rows + tile - 1) / tile;
+  return rows / tile + (groups < rows ? groups : rows);
+}
+
 template <bool kSwap, int kCols>
 void product(const ScaledView& a, const BlocksView& w, const Params& p, int sms, cudaStream_t s) {
   using S = Shape<kSwap, kCols>;
@@ -552,11 +558,8 @@ void product(const ScaledView& a, const BlocksView& w, const Params& p, int sms,
     const int b = p.type == kF32 ? 4 : 2;
     my = map_of(p.y, p.n, p.rows, p.ldy * b, 1, 0, 32, 2, b);
   }
-  // the most tiles that the groups' sizes allow
   const long long n_tiles = (p.n + S::kNTile - 1) / S::kNTile;
-  const long long row_tiles =
-      p.rows / S::kRowTile + (w.groups < p.rows ? w.groups : (long long)p.rows);
-  const long long tiles = row_tiles * n_tiles;
+  const long long tiles = row_tiles_for(p.rows, p.groups, S::kRowTile) * n_tiles;
   if (tiles > INT_MAX - sms) throw LaunchFailed{cudaErrorInvalidValue};   // no memory holds such a Y
   int splits = 1;
   if (kSwap)
@@ -585,11 +588,27 @@ int launch_scaled_product(const ScaledView& a, const BlocksView& w, const int* g
   p.type = y.type;
   const int b = y.type == kF32 ? 4 : 2;
   p.vec = (uintptr_t)y.data % 16 == 0 && y.ld * b % 16 == 0;
-  const long long each = (y.rows + w.groups - 1) / w.groups;   // rows per group, if all are used
-  if (each <= 16) product<true, 16>(a, w, p, sms, s);
-  else if (each <= 32) product<true, 32>(a, w, p, sms, s);
-  else if (each <= 64) product<true, 64>(a, w, p, sms, s);
-  else if (w.rows <= 128) product<false, 128>(a, w, p, sms, s);
+  // Few rows per group: the weights as lanes, and as few columns as mostly hold a group's rows (half
+  // as many again as the mean; one group's rows are known). Else the rows as lanes, unless that
+  // leaves more than half of the SMs without a tile, where the other layout can split K. 256 columns
+  // unless 128 fill the SMs so much better that the narrower tile's waves, four fifths as long, are
+  // fewer in time. Measured, in us, as 16 | 32 | 64 columns of rows | 128 | 256 columns of weights:
+  //   64 groups, 2048 x 2048:  8 rows each  50 | 50 | 53 | 58 |  53
+  //                           16 rows each  54 | 50 | 54 | 61 |  56
+  //                           48 rows each 120 | 79 | 57 | 63 |  57
+  //                          128 rows each 276 |169 |125 | 84 |  73
+  //   one group,  4096 x 4096:  48 rows      13 | 12 | 10 | 15 |  19
+  //                            512 rows      68 | 44 | 29 | 17 |  21
+  //                           1024 rows     130 | 73 | 52 | 29 |  22
+  //   one group,  512 x 2048:  128 rows       9 |  7 |  7 | 10 |  13
+  const long long fits = p.groups == 1 ? p.rows : p.rows * 3ll / 2 / p.groups;
+  const long long row_tiles = row_tiles_for(p.rows, p.groups, kLanes);
+  const long long narrow = row_tiles * ((p.n + 127) / 128), wide = row_tiles * ((p.n + 255) / 256);
+  auto waves = [&](long long tiles) { return (tiles + sms - 1) / sms; };
+  if (fits <= 16) product<true, 16>(a, w, p, sms, s);
+  else if (fits <= 32) product<true, 32>(a, w, p, sms, s);
+  else if (fits <= 64 || narrow * 2 <= sms) product<true, 64>(a, w, p, sms, s);
+  else if (waves(wide) * 5 > waves(narrow) * 4) product<false, 128>(a, w, p, sms, s);
   else product<false, 256>(a, w, p, sms, s);
   return 1;
 }
