@@ -3,8 +3,8 @@
 //   scale = max(amax / 448, smallest normal float),   q = e4m3(value / scale)
 //
 // value is X, or silu(X[:, :n]) X[:, n:]; for dispatch, a token's row is quantised once and
-// written to each of its pairs' rows. 8 lanes hold a block, 16 neighbouring columns each; the
-// largest magnitude is a maximum that keeps a NaN. The quotients are rounded as divisions are (a
+// written to each of its pairs' rows. The largest magnitude of a block is
+// a maximum over its lanes that keeps a NaN. The quotients are rounded as divisions are (a
 // product with the reciprocal would round differently), at three instructions each.
 //
 // Bound by memory, but only just: at 25 (gated) instructions per element the SMs issue 70 % of
@@ -22,25 +22,40 @@ namespace appt {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPer = 16;                              // columns of a lane
-constexpr int kLanes = kScaleBlock / kPer;            // lanes of a block
-constexpr int kBlocksPerCta = kThreads / kLanes;
 
-// n of a lane's 16 values, zeros behind them; n is 16 or 0 where kVec.
+// How a block's columns lie in its lanes. kVec: 8 lanes of 16 neighbouring columns, moved as 16-byte
+// words. Else (rows that do not start on 16 bytes) 32 lanes of 4 columns that are 32 apart, so that
+// the lanes' single elements are neighbours.
+template <bool kVec>
+struct Lay {
+  static constexpr int kLanes = kVec ? 8 : 32;
+  static constexpr int kPer = kScaleBlock / kLanes;
+  static constexpr int kBlocksPerCta = kThreads / kLanes;
+  // column of a lane's i-th value in the block
+  static __device__ __forceinline__ int col(int lane, int i) {
+    return kVec ? lane * kPer + i : i * kLanes + lane;
+  }
+};
+
+// A lane's values of a block of which the first n columns exist (kVec: all or none of a lane's);
+// zeros for the others.
 template <bool kVec, typename T>
-__device__ __forceinline__ void load16(const T* p, int n, float (&v)[kPer]) {
+__device__ __forceinline__ void load_block(const T* p, int lane, int n,
+                                           float (&v)[Lay<kVec>::kPer]) {
+  using L = Lay<kVec>;
   if constexpr (kVec) {
     constexpr int N = 16 / sizeof(T);
 #pragma unroll
-    for (int i = 0; i < kPer; i += N) {
+    for (int i = 0; i < L::kPer; i += N) {
       float f[N] = {};
-      if (n) ((const Pack<T, N>*)(p + i))->up(f);
+      if (L::col(lane, 0) < n) ((const Pack<T, N>*)(p + L::col(lane, i)))->up(f);
 #pragma unroll
       for (int k = 0; k < N; ++k) v[i + k] = f[k];
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) v[i] = i < n ? Value<T>::up(p[i]) : 0.f;
+    for (int i = 0; i < L::kPer; ++i)
+      v[i] = L::col(lane, i) < n ? Value<T>::up(p[L::col(lane, i)]) : 0.f;
   }
 }
 
@@ -85,14 +100,17 @@ struct Target {
   int ld, scale_ld, rows;
 };
 
-template <bool kVec>
-__device__ __forceinline__ void store16(unsigned char* p, int n, const unsigned (&q)[4]) {
+template <bool kVec, int kWords>
+__device__ __forceinline__ void store_block(unsigned char* p, int lane, int n,
+                                            const unsigned (&q)[kWords]) {
+  using L = Lay<kVec>;
   if constexpr (kVec) {
-    if (n) *(uint4*)p = make_uint4(q[0], q[1], q[2], q[3]);
+    if (L::col(lane, 0) < n)
+      *(uint4*)(p + L::col(lane, 0)) = make_uint4(q[0], q[1], q[2], q[3]);
   } else {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (i < n) p[i] = (unsigned char)(q[i / 4] >> (8 * (i % 4)));
+    for (int i = 0; i < L::kPer; ++i)
+      if (L::col(lane, i) < n) p[L::col(lane, i)] = (unsigned char)(q[0] >> (8 * i));
   }
 }
 
@@ -101,16 +119,19 @@ __device__ __forceinline__ unsigned e4m3x2(float lo, float hi) {
 }
 
 // kVec: every row of X (its gate's half too) and of Q starts on 16 bytes, and the columns are a
-// multiple of 16. 2^groups_log2 groups of 8 lanes work on a row.
+// multiple of 16. 2^groups_log2 groups of a block's lanes work on a row.
 template <typename T, bool kGated, bool kRouted, bool kVec>
 __global__ void __launch_bounds__(kThreads)
     quantize_kernel(const T* __restrict__ x, long long ldx, long long rows,
                     const int* __restrict__ rows_ptr, const int* __restrict__ pair_row, int top_k,
                     int groups_log2, Target o) {
-  const int sub = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
-  const unsigned mine = 0xffu << (threadIdx.x & 24);   // the block's lanes
+  using L = Lay<kVec>;
+  constexpr int kPer = L::kPer;
+  const int sub = threadIdx.x % L::kLanes, group = threadIdx.x / L::kLanes;
+  // the block's lanes
+  const unsigned mine = kVec ? 0xffu << (threadIdx.x & 24) : kFull;
   const int blocks = (int)((o.cols + kScaleBlock - 1) / kScaleBlock);
-  const int step = 1 << groups_log2, per_cta = kBlocksPerCta >> groups_log2;
+  const int step = 1 << groups_log2, per_cta = L::kBlocksPerCta >> groups_log2;
   if (!kRouted && rows_ptr) {
     const long long r = *rows_ptr;
     rows = r < rows ? (r > 0 ? r : 0) : rows;
@@ -118,14 +139,14 @@ __global__ void __launch_bounds__(kThreads)
   for (long long row = (long long)blockIdx.x * per_cta + (group >> groups_log2); row < rows;
        row += (long long)gridDim.x * per_cta) {
     for (int block = group & (step - 1); block < blocks; block += step) {
-      const long long col = (long long)block * kScaleBlock + sub * kPer;
-      const int n = col < o.cols ? (o.cols - col < kPer ? (int)(o.cols - col) : kPer) : 0;
+      const long long col = (long long)block * kScaleBlock;
+      const int n = o.cols - col < kScaleBlock ? (int)(o.cols - col) : kScaleBlock;
       const T* p = x + row * ldx + col;
       float v[kPer];
-      load16<kVec>(p, n, v);
+      load_block<kVec>(p, sub, n, v);
       if (kGated) {
         float up[kPer];
-        load16<kVec>(p + o.cols, n, up);
+        load_block<kVec>(p + o.cols, sub, n, up);
 #pragma unroll
         for (int k = 0; k < kPer; ++k) v[k] = silu(v[k]) * up[k];
       }
@@ -133,20 +154,20 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
       for (int k = 0; k < kPer; k += 2) top = abs_max(v[k], v[k + 1], top);
 #pragma unroll
-      for (int s = kLanes / 2; s > 0; s >>= 1)
+      for (int s = L::kLanes / 2; s > 0; s >>= 1)
         top = abs_max(__shfl_xor_sync(mine, top, s), 0.f, top);
       float scale = __fdiv_rn(top, 448.f);
       if (scale < FLT_MIN) scale = FLT_MIN;   // false for NaN
       const Divisor div(scale);
-      unsigned q[4];
+      unsigned q[kPer / 4];
       if (div.holds()) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < kPer / 4; ++k)
           q[k] = e4m3x2(div.of(v[4 * k]), div.of(v[4 * k + 1])) |
                  e4m3x2(div.of(v[4 * k + 2]), div.of(v[4 * k + 3])) << 16;
       } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < kPer / 4; ++k)
           q[k] = e4m3x2(__fdiv_rn(v[4 * k], scale), __fdiv_rn(v[4 * k + 1], scale)) |
                  e4m3x2(__fdiv_rn(v[4 * k + 2], scale), __fdiv_rn(v[4 * k + 3], scale)) << 16;
       }
@@ -161,12 +182,12 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if ((unsigned)r[j] >= (unsigned)o.rows) continue;
-            store16<kVec>(pq + (long long)r[j] * o.ld, n, q);
+            store_block<kVec>(pq + (long long)r[j] * o.ld, sub, n, q);
             if (sub == 0) ps[r[j]] = scale;
           }
         }
       } else {
-        store16<kVec>(o.q + row * o.ld + col, n, q);
+        store_block<kVec>(o.q + row * o.ld + col, sub, n, q);
         if (sub == 0) ps[row] = scale;
       }
     }
@@ -178,6 +199,7 @@ void quantize(const DenseView& x, bool gated, const int* rows_ptr, const RoutesV
               const Target& o, cudaStream_t s) {
   const long long blocks = (o.cols + kScaleBlock - 1) / kScaleBlock;
   int groups = 0;   // no more than a row has blocks
+  constexpr int kBlocksPerCta = Lay<kVec>::kBlocksPerCta;
   while (2 << groups <= kBlocksPerCta && 2 << groups <= blocks) ++groups;
   const int per_cta = kBlocksPerCta >> groups;
   const long long ctas = (x.rows + per_cta - 1) / per_cta;
@@ -198,7 +220,7 @@ template <typename T>
 void quantize(const DenseView& x, bool gated, const int* rows_ptr, const RoutesView* routes,
               const Target& o, cudaStream_t s) {
   const bool vec = (uintptr_t)x.data % 16 == 0 && x.ld * sizeof(T) % 16 == 0 &&
-                   (uintptr_t)o.q % 16 == 0 && o.ld % 16 == 0 && o.cols % kPer == 0;
+                   (uintptr_t)o.q % 16 == 0 && o.ld % 16 == 0 && o.cols % 16 == 0;
   if (vec) quantize<T, true>(x, gated, rows_ptr, routes, o, s);
   else quantize<T, false>(x, gated, rows_ptr, routes, o, s);
 }

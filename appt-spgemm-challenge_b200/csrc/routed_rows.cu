@@ -17,9 +17,10 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Pieces that a thread of dispatch has in flight: 64 bytes, or 8 single elements where rows do not
-// start and end on 16 bytes.
-__host__ __device__ constexpr int pieces_in_flight(int elements) { return elements > 1 ? 4 : 8; }
+// Pieces that a thread has in flight. A piece is 16 bytes, or a single element where rows do not
+// start and end on 16 bytes: more of those.
+__host__ __device__ constexpr int dispatch_pieces(int elements) { return elements > 1 ? 4 : 8; }
+__host__ __device__ constexpr int combine_pieces(int elements) { return elements > 1 ? 1 : 4; }
 
 // What the three kernels share: `lanes` (a multiple of 32) threads per token.
 struct Shape {
@@ -59,7 +60,7 @@ __global__ void __launch_bounds__(kThreads)
                     int rows) {
   using A = typename Value<T>::Acc;
   using P = Pack<T, N>;
-  constexpr int U = pieces_in_flight(N);
+  constexpr int U = dispatch_pieces(N);
   const Place me = place(s);
   if (me.token < 0) return;   // whole warps
   const P* px = (const P*)(x + (long long)me.token * ldx);
@@ -102,49 +103,57 @@ __global__ void __launch_bounds__(kThreads)
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads)
     combine_kernel(Shape s, const T* __restrict__ h, int ldh, int rows,
-                   const typename Value<T>::Acc* __restrict__ w, T* __restrict__ y,
-                   int ldy) {
+                   const typename Value<T>::Acc* __restrict__ w, T* __restrict__ y, int ldy) {
   using A = typename Value<T>::Acc;
   using P = Pack<T, N>;
   constexpr int J = 4;   // rows in flight
+  constexpr int U = combine_pieces(N);
   const Place me = place(s);
   if (me.token < 0) return;
   P* py = (P*)(y + (long long)me.token * ldy);
-  for (long long base = (long long)blockIdx.y * s.lanes; base < s.pieces;
-       base += (long long)gridDim.y * s.lanes) {
-    const long long c = base + me.at;
-    A sum[N];
+  for (long long base = (long long)blockIdx.y * s.lanes * U; base < s.pieces;
+       base += (long long)gridDim.y * s.lanes * U) {
+    const long long c0 = base + me.at;
+    A sum[U][N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) sum[i] = A(0);
+    for (int k = 0; k < U; ++k)
+#pragma unroll
+      for (int i = 0; i < N; ++i) sum[k][i] = A(0);
     for (int j0 = 0; j0 < s.top_k; j0 += 32) {
       const int mine = lane_row(s, me.token, j0, rows);
       const A wmine = lane_weight(s, w, me.token, j0, mine);
       for (int j = 0; j < 32 && j0 + j < s.top_k; j += J) {
-        P v[J];
+        P v[J][U];
         int row[J];
         A wj[J];
 #pragma unroll
         for (int u = 0; u < J; ++u) {
           row[u] = __shfl_sync(kFull, mine, (j + u) & 31);   // lanes past top_k hold -1
           wj[u] = __shfl_sync(kFull, wmine, (j + u) & 31);
-          if (row[u] >= 0 && c < s.pieces) v[u] = ((const P*)(h + (long long)row[u] * ldh))[c];
+          const P* ph = (const P*)(h + (long long)row[u] * ldh) + c0;
+#pragma unroll
+          for (int k = 0; k < U; ++k)
+            if (row[u] >= 0 && c0 + k * s.lanes < s.pieces) v[u][k] = ph[k * s.lanes];
         }
-        if (c < s.pieces) {
 #pragma unroll
-          for (int u = 0; u < J; ++u) {
-            if (row[u] < 0) continue;
+        for (int u = 0; u < J; ++u) {
+#pragma unroll
+          for (int k = 0; k < U; ++k) {
+            if (row[u] < 0 || c0 + k * s.lanes >= s.pieces) continue;
             A f[N];
-            v[u].up(f);
+            v[u][k].up(f);
 #pragma unroll
-            for (int i = 0; i < N; ++i) sum[i] += wj[u] * f[i];
+            for (int i = 0; i < N; ++i) sum[k][i] += wj[u] * f[i];
           }
         }
       }
     }
-    if (c < s.pieces) {
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      if (c0 + k * s.lanes >= s.pieces) continue;
       P o;
-      o.down(sum);
-      py[c] = o;
+      o.down(sum[k]);
+      py[c0 + k * s.lanes] = o;
     }
   }
 }
@@ -153,14 +162,14 @@ __global__ void __launch_bounds__(kThreads)
 // one group of threads, J pairs at a time, and are summed in a fixed order (over a thread's
 // pieces, over the lanes, over the warps).
 template <typename T, int N>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, N > 1 ? 4 : sizeof(T) == 8 ? 2 : 3)
     combine_grad_kernel(Shape s, const T* __restrict__ dy, int ldy, const T* __restrict__ h,
-                        int ldh, int rows,
-                        const typename Value<T>::Acc* __restrict__ w, T* __restrict__ dh,
-                        int lddh, typename Value<T>::Acc* __restrict__ dw) {
+                        int ldh, int rows, const typename Value<T>::Acc* __restrict__ w,
+                        T* __restrict__ dh, int lddh, typename Value<T>::Acc* __restrict__ dw) {
   using A = typename Value<T>::Acc;
   using P = Pack<T, N>;
   constexpr int J = 4;
+  constexpr int U = combine_pieces(N);
   __shared__ A part[kThreads / 32][J];
   const Place me = place(s);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -179,28 +188,39 @@ __global__ void __launch_bounds__(kThreads)
       dot[u] = A(0);
     }
     if (me.token >= 0) {
-      for (long long c = me.at; c < s.pieces; c += s.lanes) {
-        A g[N];
-        py[c].up(g);
-        P v[J];
+      for (long long c = me.at; c < s.pieces; c += (long long)s.lanes * U) {
+        P g[U], v[J][U];
 #pragma unroll
-        for (int u = 0; u < J; ++u)
-          if (dw && row[u] >= 0) v[u] = ((const P*)(h + (long long)row[u] * ldh))[c];
+        for (int k = 0; k < U; ++k)
+          if (c + k * s.lanes < s.pieces) g[k] = py[c + k * s.lanes];
 #pragma unroll
         for (int u = 0; u < J; ++u) {
-          if (row[u] < 0) continue;
-          A f[N];
-          if (dw) {
-            v[u].up(f);
+          const P* ph = (const P*)(h + (long long)row[u] * ldh) + c;
 #pragma unroll
-            for (int i = 0; i < N; ++i) dot[u] += g[i] * f[i];
-          }
-          if (dh) {
+          for (int k = 0; k < U; ++k)
+            if (dw && row[u] >= 0 && c + k * s.lanes < s.pieces) v[u][k] = ph[k * s.lanes];
+        }
 #pragma unroll
-            for (int i = 0; i < N; ++i) f[i] = wj[u] * g[i];
-            P o;
-            o.down(f);
-            ((P*)(dh + (long long)row[u] * lddh))[c] = o;
+        for (int k = 0; k < U; ++k) {
+          if (c + k * s.lanes >= s.pieces) continue;
+          A gf[N];
+          g[k].up(gf);
+#pragma unroll
+          for (int u = 0; u < J; ++u) {
+            if (row[u] < 0) continue;
+            A f[N];
+            if (dw) {
+              v[u][k].up(f);
+#pragma unroll
+              for (int i = 0; i < N; ++i) dot[u] += gf[i] * f[i];
+            }
+            if (dh) {
+#pragma unroll
+              for (int i = 0; i < N; ++i) f[i] = wj[u] * gf[i];
+              P o;
+              o.down(f);
+              ((P*)(dh + (long long)row[u] * lddh))[c + k * s.lanes] = o;
+            }
           }
         }
       }
@@ -226,9 +246,10 @@ bool wide(const DenseView& m, int bytes) {
   return (uintptr_t)m.data % 16 == 0 && m.ld * bytes % 16 == 0;
 }
 
-Shape shape_for(const RoutesView& r, int pieces) {
+// As many threads per token as its pieces keep busy, `each` per thread.
+Shape shape_for(const RoutesView& r, int pieces, int each) {
   Shape s{r.pair_row, r.tokens, r.top_k, pieces, 32};
-  while (s.lanes < kThreads && s.lanes < pieces) s.lanes *= 2;
+  while (s.lanes < kThreads && (long long)s.lanes * each < pieces) s.lanes *= 2;
   return s;
 }
 
@@ -271,8 +292,8 @@ int launch_dispatch(const RoutesView& r, const DenseView& x, const void* w, cons
   by_type(x.type, x.cols, wide(x, b) && wide(y, b), [&](auto t, auto n) {
     using T = decltype(t);
     constexpr int N = decltype(n)::value;
-    const Shape sh = shape_for(r, (int)(x.cols / N));
-    launch(nullptr, dispatch_kernel<T, N>, grid_for(sh, sh.lanes * pieces_in_flight(N)), kThreads, 0, s, 1, sh,
+    const Shape sh = shape_for(r, (int)(x.cols / N), dispatch_pieces(N));
+    launch(nullptr, dispatch_kernel<T, N>, grid_for(sh, sh.lanes * dispatch_pieces(N)), kThreads, 0, s, 1, sh,
            (const T*)x.data, x.ld, (const typename Value<T>::Acc*)w, (T*)y.data, y.ld, y.rows);
   });
   return 1;
@@ -285,8 +306,8 @@ int launch_combine(const RoutesView& r, const DenseView& h, const void* w, const
   by_type(h.type, h.cols, wide(h, b) && wide(y, b), [&](auto t, auto n) {
     using T = decltype(t);
     constexpr int N = decltype(n)::value;
-    const Shape sh = shape_for(r, (int)(h.cols / N));
-    launch(nullptr, combine_kernel<T, N>, grid_for(sh, sh.lanes), kThreads, 0, s, 1, sh,
+    const Shape sh = shape_for(r, (int)(h.cols / N), combine_pieces(N));
+    launch(nullptr, combine_kernel<T, N>, grid_for(sh, sh.lanes * combine_pieces(N)), kThreads, 0, s, 1, sh,
            (const T*)h.data, h.ld, h.rows, (const typename Value<T>::Acc*)w, (T*)y.data, y.ld);
   });
   return 1;
@@ -301,7 +322,7 @@ int launch_combine_grad(const RoutesView& r, const DenseView& dy, const DenseVie
     using T = decltype(t);
     using A = typename Value<T>::Acc;
     constexpr int N = decltype(n)::value;
-    const Shape sh = shape_for(r, (int)(dy.cols / N));
+    const Shape sh = shape_for(r, (int)(dy.cols / N), combine_pieces(N));
     const int per = kThreads / sh.lanes;
     launch(nullptr, combine_grad_kernel<T, N>, (r.tokens + per - 1) / per, kThreads, 0, s, 1, sh,
            (const T*)dy.data, dy.ld, h ? (const T*)h->data : nullptr, h ? h->ld : 0,

@@ -101,6 +101,30 @@ __device__ __forceinline__ void store_one(const Params& p, long long at, float v
   else ((__nv_bfloat16*)p.y)[at] = __float2bfloat16_rn(v);
 }
 
+// The first `rows` rows and `left_cols` columns of a warp's boxes to Y; not inlined, for it would
+// take registers that the sums need.
+template <typename T, int kBoxes>
+__device__ __noinline__ void store_boxes(T* y, long long ldy, bool vec, const char* boxes, int rows,
+                                         int left_cols) {
+  constexpr int kPer = 16 / sizeof(T), kPieces = 8 * kBoxes;
+  const int lane = threadIdx.x & 31, cols = min(left_cols, kPieces * kPer);
+  auto piece = [&](int r, int j) {
+    return (const T*)(boxes + j / 8 * kOutBox + r * 128 + ((j % 8) ^ (r & 7)) * 16);
+  };
+  if (vec) {
+    const int j = lane % kPieces, left = cols - j * kPer;
+    for (int r = lane / kPieces; r < rows; r += 32 / kPieces) {
+      T* to = y + r * ldy + j * kPer;
+      if (left >= kPer) *(uint4*)to = *(const uint4*)piece(r, j);
+      else
+        for (int i = 0; i < left; ++i) to[i] = piece(r, j)[i];
+    }
+  } else {
+    for (int r = 0; r < rows; ++r)
+      for (int c = lane; c < cols; c += 32) y[r * ldy + c] = piece(r, c / kPer)[c % kPer];
+  }
+}
+
 // A warp's 32 rows x N columns of Y, a row per thread, through boxes in shared memory that TMA
 // copies while the warp goes on with its next tile. The 16-byte pieces of a row change places by
 // the row (the 128-byte swizzle), which spreads the threads over the banks. Stores from registers
@@ -109,7 +133,7 @@ __device__ __forceinline__ void store_one(const Params& p, long long at, float v
 template <typename T, int N, int kBoxes>
 __device__ __forceinline__ void write_rows(const Params& p, const CUtensorMap* map, char* boxes,
                                            const uint64_t* v, int row, int rows, int n) {
-  constexpr int kPer = 16 / sizeof(T), kCols = 128 / sizeof(T), kPieces = 8 * kBoxes;
+  constexpr int kPer = 16 / sizeof(T), kCols = 128 / sizeof(T);
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int c0 = 0; c0 < N; c0 += kBoxes * kCols) {   // once, or twice for 32 bits
@@ -136,17 +160,8 @@ __device__ __forceinline__ void write_rows(const Params& p, const CUtensorMap* m
       }
     } else {
       __syncwarp();
-      const int j = lane % kPieces, c = c0 + j * kPer, cols = p.n - n - c;
-      for (int r = lane / kPieces; r < min(rows, 32); r += 32 / kPieces) {
-        const T* from =
-            (const T*)(boxes + j / 8 * kOutBox + r * 128 + ((j % 8) ^ (r & 7)) * 16);
-        T* y = (T*)p.y + (row + r) * p.ldy + n + c;
-        if (p.vec && cols >= kPer) {
-          *(uint4*)y = *(const uint4*)from;
-        } else {
-          for (int i = 0; i < min(cols, kPer); ++i) y[i] = from[i];
-        }
-      }
+      store_boxes<T, kBoxes>((T*)p.y + (long long)row * p.ldy + n + c0, p.ldy, p.vec, boxes,
+                             min(rows, 32), p.n - n - c0);
     }
   }
 }
@@ -563,7 +578,9 @@ void product(const ScaledView& a, const BlocksView& w, const Params& p, int sms,
   if (tiles > INT_MAX - sms) throw LaunchFailed{cudaErrorInvalidValue};   // no memory holds such a Y
   int splits = 1;
   if (kSwap)
-    while (splits < 8 && tiles * splits * 2 <= sms && splits * 2 <= p.k_blocks) splits *= 2;
+    // (a cluster's CTAs share a GPC, whose SMs the clusters may not all fill: a second wave of
+    // them took 13.7 us where 7 was expected)
+    while (splits < 8 && tiles * splits * 2 <= sms * 7 / 8 && splits * 2 <= p.k_blocks) splits *= 2;
   const long long ctas = splits > 1 ? tiles * splits : tiles < sms ? tiles : sms;
   launch(&opted, product_kernel<kSwap, kCols>, dim3((unsigned)ctas), dim3(S::kThreads), S::kBytes, s,
          splits, ma, mw, my, p, splits);
