@@ -4,6 +4,10 @@ Tolerances count roundings: u(t) = finfo(t).eps / 2 is the half step of a type, 
 smallest subnormal step; a sum of n terms in a type of half step u is off by at most n u times the
 sum of the terms' magnitudes, in whatever order it is taken.
 """
+import subprocess
+import sys
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
@@ -125,6 +129,29 @@ def test_route_of_strided_ids_and_far_ids():
     ids[::5, 1] += 1 << 32      # equal to a valid id in its low 32 bits
     _, *out = route(ids, 16)
     check_route(ids, 16, *out)
+
+
+FIRST_CALLS = """
+import sys
+sys.path[:0] = {paths!r}
+import numpy as np
+import test_experts_gpu as t
+for tokens in (100, 2000, 40000):
+    ids = t.ids_for(t.gen(1), tokens, 4, {experts}, "wild")
+    _, *out = t.route(ids, {experts})
+    t.check_route(ids, {experts}, *out)
+print("ok")
+"""
+
+
+@pytest.mark.parametrize("experts", [300, 340, 420])
+def test_route_as_a_process_s_first_call(experts):
+    """Shared memory between what every kernel may have and the most: the opt-in is a kernel's own
+    and must not come from an earlier, larger call."""
+    code = FIRST_CALLS.format(paths=[str(Path(__file__).parent), *map(str, sys.path)],
+                              experts=experts)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "ok" in r.stdout, r.stderr[-2000:]
 
 
 # --------------------------------------------------------------------------- rows there and back
