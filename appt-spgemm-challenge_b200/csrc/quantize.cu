@@ -7,10 +7,11 @@
 // a maximum over its lanes that keeps a NaN. The quotients are rounded as divisions are (a
 // product with the reciprocal would round differently), at three instructions each.
 //
-// Bound by memory, but only just: at 25 (gated) instructions per element the SMs issue 70 % of
-// what they can. Gated bf16 16384 x 2048: 33 us, 5.1 TB/s (16-bit access, plain divisions and
-// 64-bit index arithmetic: 74 us). Routed bf16 8192 x 4096 to 8 experts each: 66 us, 5.2 TB/s (84
-// us); the scales' 4-byte writes land in rows far apart.
+// Bound by memory, but only just: some 25 (gated) instructions per element are 70 % of what the SMs
+// can issue. Gated bf16 16384 x 2048: 30 us, 5.6 TB/s (with both operands unpacked as they arrive 37,
+// with plain divisions, exponentials and 64-bit index arithmetic 74). Routed bf16 8192 x 4096 to 8
+// experts each: 63 us, 5.5 TB/s (84 us); the scales' 4-byte writes land in rows far apart. Rows that
+// do not start on 16 bytes take twice as long: 2047 columns gated 58 us.
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <cfloat>
@@ -23,41 +24,43 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// How a block's columns lie in its lanes. kVec: 8 lanes of 16 neighbouring columns, moved as 16-byte
-// words. Else (rows that do not start on 16 bytes) 32 lanes of 4 columns that are 32 apart, so that
-// the lanes' single elements are neighbours.
-template <bool kVec>
+// How a block's columns lie in its lanes. kVec: 8 lanes of 16 neighbouring columns (32 bits: 16 lanes
+// of 8, so that a lane's 16-byte words are two neighbours of another lane's), moved as such. Else (rows that do not start on 16 bytes) 32 lanes of 4 neighbouring columns, read one by
+// one, and stored as a word where rows of Q start on 4 bytes.
+template <typename T, bool kVec>
 struct Lay {
-  static constexpr int kLanes = kVec ? 8 : 32;
+  static constexpr int kLanes = !kVec ? 32 : sizeof(T) == 4 ? 16 : 8;
   static constexpr int kPer = kScaleBlock / kLanes;
   static constexpr int kBlocksPerCta = kThreads / kLanes;
   // column of a lane's i-th value in the block
-  static __device__ __forceinline__ int col(int lane, int i) {
-    return kVec ? lane * kPer + i : i * kLanes + lane;
-  }
+  static __device__ __forceinline__ int col(int lane, int i) { return lane * kPer + i; }
 };
 
-// A lane's values of a block of which the first n columns exist (kVec: all or none of a lane's);
-// zeros for the others.
-template <bool kVec, typename T>
-__device__ __forceinline__ void load_block(const T* p, int lane, int n,
-                                           float (&v)[Lay<kVec>::kPer]) {
-  using L = Lay<kVec>;
-  if constexpr (kVec) {
-    constexpr int N = 16 / sizeof(T);
+// A lane's values of a block of which the first n columns exist (kVec: all or none of a lane's),
+// zeros for the others: fetched, and unpacked later, so that a gate and its factor are on their way
+// together.
+template <typename T, bool kVec>
+struct Values {
+  using L = Lay<T, kVec>;
+  static constexpr int N = kVec ? 16 / sizeof(T) : 1;
+  Pack<T, N> raw[L::kPer / N];
+  __device__ __forceinline__ void fetch(const T* p, int lane, int n) {
 #pragma unroll
-    for (int i = 0; i < L::kPer; i += N) {
-      float f[N] = {};
-      if (L::col(lane, 0) < n) ((const Pack<T, N>*)(p + L::col(lane, i)))->up(f);
-#pragma unroll
-      for (int k = 0; k < N; ++k) v[i + k] = f[k];
+    for (int i = 0; i < L::kPer / N; ++i) {
+      raw[i] = Pack<T, N>{};
+      if (L::col(lane, kVec ? 0 : i) < n) raw[i] = *(const Pack<T, N>*)(p + L::col(lane, i * N));
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < L::kPer; ++i)
-      v[i] = L::col(lane, i) < n ? Value<T>::up(p[L::col(lane, i)]) : 0.f;
   }
-}
+  __device__ __forceinline__ void unpack(float (&v)[L::kPer]) const {
+#pragma unroll
+    for (int i = 0; i < L::kPer / N; ++i) {
+      float f[N];
+      raw[i].up(f);
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[i * N + k] = f[k];
+    }
+  }
+};
 
 // x / s in fp32, rounded to nearest as a division is, for many x with one s: with y the rounded
 // reciprocal and q = x y, one step q + (x - q s) y corrects the last place (Markstein's method; the
@@ -98,19 +101,24 @@ struct Target {
   float* scale;
   long long cols;
   int ld, scale_ld, rows;
+  bool words;   // rows of q start on 4 bytes
 };
 
+// A lane's 4 kWords values; words: rows of q start on 4 bytes (on 16 where kVec).
 template <bool kVec, int kWords>
 __device__ __forceinline__ void store_block(unsigned char* p, int lane, int n,
-                                            const unsigned (&q)[kWords]) {
-  using L = Lay<kVec>;
+                                            const unsigned (&q)[kWords], bool words) {
+  const int c = lane * 4 * kWords;
   if constexpr (kVec) {
-    if (L::col(lane, 0) < n)
-      *(uint4*)(p + L::col(lane, 0)) = make_uint4(q[0], q[1], q[2], q[3]);
+    if (c >= n) return;
+    if constexpr (kWords == 4) *(uint4*)(p + c) = make_uint4(q[0], q[1], q[2], q[3]);
+    else *(uint2*)(p + c) = make_uint2(q[0], q[1]);
+  } else if (words && c + 3 < n) {
+    *(unsigned*)(p + c) = q[0];
   } else {
 #pragma unroll
-    for (int i = 0; i < L::kPer; ++i)
-      if (L::col(lane, i) < n) p[L::col(lane, i)] = (unsigned char)(q[0] >> (8 * i));
+    for (int i = 0; i < 4; ++i)
+      if (c + i < n) p[c + i] = (unsigned char)(q[0] >> (8 * i));
   }
 }
 
@@ -121,15 +129,17 @@ __device__ __forceinline__ unsigned e4m3x2(float lo, float hi) {
 // kVec: every row of X (its gate's half too) and of Q starts on 16 bytes, and the columns are a
 // multiple of 16. 2^groups_log2 groups of a block's lanes work on a row.
 template <typename T, bool kGated, bool kRouted, bool kVec>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 5)
     quantize_kernel(const T* __restrict__ x, long long ldx, long long rows,
                     const int* __restrict__ rows_ptr, const int* __restrict__ pair_row, int top_k,
                     int groups_log2, Target o) {
-  using L = Lay<kVec>;
+  using L = Lay<T, kVec>;
   constexpr int kPer = L::kPer;
   const int sub = threadIdx.x % L::kLanes, group = threadIdx.x / L::kLanes;
   // the block's lanes
-  const unsigned mine = kVec ? 0xffu << (threadIdx.x & 24) : kFull;
+  const unsigned mine = L::kLanes == 32
+                            ? kFull
+                            : ((1u << L::kLanes % 32) - 1) << (threadIdx.x & 31 & -L::kLanes);
   const int blocks = (int)((o.cols + kScaleBlock - 1) / kScaleBlock);
   const int step = 1 << groups_log2, per_cta = L::kBlocksPerCta >> groups_log2;
   if (!kRouted && rows_ptr) {
@@ -142,11 +152,14 @@ __global__ void __launch_bounds__(kThreads)
       const long long col = (long long)block * kScaleBlock;
       const int n = o.cols - col < kScaleBlock ? (int)(o.cols - col) : kScaleBlock;
       const T* p = x + row * ldx + col;
+      Values<T, kVec> in, factor;
+      in.fetch(p, sub, n);
+      if (kGated) factor.fetch(p + o.cols, sub, n);
       float v[kPer];
-      load_block<kVec>(p, sub, n, v);
+      in.unpack(v);
       if (kGated) {
         float up[kPer];
-        load_block<kVec>(p + o.cols, sub, n, up);
+        factor.unpack(up);
 #pragma unroll
         for (int k = 0; k < kPer; ++k) v[k] = silu(v[k]) * up[k];
       }
@@ -182,12 +195,12 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if ((unsigned)r[j] >= (unsigned)o.rows) continue;
-            store_block<kVec>(pq + (long long)r[j] * o.ld, sub, n, q);
+            store_block<kVec>(pq + (long long)r[j] * o.ld, sub, n, q, o.words);
             if (sub == 0) ps[r[j]] = scale;
           }
         }
       } else {
-        store_block<kVec>(o.q + row * o.ld + col, sub, n, q);
+        store_block<kVec>(o.q + row * o.ld + col, sub, n, q, o.words);
         if (sub == 0) ps[row] = scale;
       }
     }
@@ -199,7 +212,7 @@ void quantize(const DenseView& x, bool gated, const int* rows_ptr, const RoutesV
               const Target& o, cudaStream_t s) {
   const long long blocks = (o.cols + kScaleBlock - 1) / kScaleBlock;
   int groups = 0;   // no more than a row has blocks
-  constexpr int kBlocksPerCta = Lay<kVec>::kBlocksPerCta;
+  constexpr int kBlocksPerCta = Lay<T, kVec>::kBlocksPerCta;
   while (2 << groups <= kBlocksPerCta && 2 << groups <= blocks) ++groups;
   const int per_cta = kBlocksPerCta >> groups;
   const long long ctas = (x.rows + per_cta - 1) / per_cta;
@@ -231,7 +244,7 @@ int launch_quantize(const DenseView& x, bool gated, const int* rows_ptr, const R
                     const ScaledView& q, cudaStream_t s) {
   if (x.rows == 0 || q.q.cols == 0 || q.q.rows == 0) return 0;
   const Target o{(unsigned char*)q.q.data, q.scale, q.q.cols, (int)q.q.ld, (int)q.scale_ld,
-                 (int)q.q.rows};
+                 (int)q.q.rows, (uintptr_t)q.q.data % 4 == 0 && q.q.ld % 4 == 0};
   switch (x.type) {
     case kF32: quantize<float>(x, gated, rows_ptr, routes, o, s); break;
     case kF16: quantize<__half>(x, gated, rows_ptr, routes, o, s); break;

@@ -8,6 +8,7 @@
 // All are bound by memory: a few operations per element. Each goes by tokens, so that a token's
 // row is read (or written) once for its k pairs, and each thread moves 16-byte pieces.
 #include <cuda_runtime.h>
+#include <algorithm>
 #include "common.cuh"
 #include "experts.h"
 #include "values.cuh"
@@ -17,10 +18,10 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Pieces that a thread has in flight. A piece is 16 bytes, or a single element where rows do not
-// start and end on 16 bytes: more of those.
-__host__ __device__ constexpr int dispatch_pieces(int elements) { return elements > 1 ? 4 : 8; }
-__host__ __device__ constexpr int combine_pieces(int elements) { return elements > 1 ? 1 : 4; }
+// Pieces that a thread has in flight. A piece is 16 bytes, or 8 or 4 or a single element where rows
+// do not start and end on 16 bytes: more of those.
+__host__ __device__ constexpr int dispatch_pieces(int bytes) { return bytes == 16 ? 4 : 8; }
+__host__ __device__ constexpr int combine_pieces(int bytes) { return bytes == 16 ? 1 : 4; }
 
 // What the three kernels share: `lanes` (a multiple of 32) threads per token.
 struct Shape {
@@ -60,7 +61,7 @@ __global__ void __launch_bounds__(kThreads)
                     int rows) {
   using A = typename Value<T>::Acc;
   using P = Pack<T, N>;
-  constexpr int U = dispatch_pieces(N);
+  constexpr int U = dispatch_pieces(N * sizeof(T));
   const Place me = place(s);
   if (me.token < 0) return;   // whole warps
   const P* px = (const P*)(x + (long long)me.token * ldx);
@@ -107,7 +108,7 @@ __global__ void __launch_bounds__(kThreads)
   using A = typename Value<T>::Acc;
   using P = Pack<T, N>;
   constexpr int J = 4;   // rows in flight
-  constexpr int U = combine_pieces(N);
+  constexpr int U = combine_pieces(N * sizeof(T));
   const Place me = place(s);
   if (me.token < 0) return;
   P* py = (P*)(y + (long long)me.token * ldy);
@@ -162,14 +163,14 @@ __global__ void __launch_bounds__(kThreads)
 // one group of threads, J pairs at a time, and are summed in a fixed order (over a thread's
 // pieces, over the lanes, over the warps).
 template <typename T, int N>
-__global__ void __launch_bounds__(kThreads, N > 1 ? 4 : sizeof(T) == 8 ? 2 : 3)
+__global__ void __launch_bounds__(kThreads, N * sizeof(T) == 16 ? 4 : sizeof(T) == 8 ? 2 : 3)
     combine_grad_kernel(Shape s, const T* __restrict__ dy, int ldy, const T* __restrict__ h,
                         int ldh, int rows, const typename Value<T>::Acc* __restrict__ w,
                         T* __restrict__ dh, int lddh, typename Value<T>::Acc* __restrict__ dw) {
   using A = typename Value<T>::Acc;
   using P = Pack<T, N>;
   constexpr int J = 4;
-  constexpr int U = combine_pieces(N);
+  constexpr int U = combine_pieces(N * sizeof(T));
   __shared__ A part[kThreads / 32][J];
   const Place me = place(s);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -242,8 +243,10 @@ __global__ void __launch_bounds__(kThreads, N > 1 ? 4 : sizeof(T) == 8 ? 2 : 3)
   }
 }
 
-bool wide(const DenseView& m, int bytes) {
-  return (uintptr_t)m.data % 16 == 0 && m.ld * bytes % 16 == 0;
+// The largest of 16, 8, 4 (and 2) bytes on which all rows of a matrix start.
+int grain(const DenseView& m, int bytes) {
+  const unsigned long long all = (uintptr_t)m.data | (unsigned long long)(m.ld * bytes);
+  return all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 2;
 }
 
 // As many threads per token as its pieces keep busy, `each` per thread.
@@ -259,25 +262,25 @@ dim3 grid_for(const Shape& s, long long per_cta_pieces) {
   return dim3((s.tokens + per - 1) / per, (unsigned)(y > 65535 ? 65535 : y));
 }
 
-// f(T{}, N): N elements per piece, 16 bytes where every row starts and ends on 16 bytes.
+template <typename T, typename F>
+void by_pieces(long long cols, int grain, F&& f) {
+  constexpr int n16 = 16 / sizeof(T), n8 = 8 / sizeof(T), n4 = 4 / sizeof(T);
+  if (grain >= 16 && cols % n16 == 0) return f(T(), std::integral_constant<int, n16>());
+  if constexpr (sizeof(T) == 4)
+    if (grain >= 8 && cols % n8 == 0) return f(T(), std::integral_constant<int, n8>());
+  if constexpr (sizeof(T) == 2)
+    if (grain >= 4 && cols % n4 == 0) return f(T(), std::integral_constant<int, n4>());
+  return f(T(), std::integral_constant<int, 1>());
+}
+
+// f(T{}, N): N elements per piece, the most that every row starts and ends on.
 template <typename F>
-void by_type(int type, long long cols, bool vec, F&& f) {
+void by_type(int type, long long cols, int grain, F&& f) {
   switch (type) {
-    case kF64:
-      if (vec && cols % 2 == 0) f(double(), std::integral_constant<int, 2>());
-      else f(double(), std::integral_constant<int, 1>());
-      break;
-    case kF32:
-      if (vec && cols % 4 == 0) f(float(), std::integral_constant<int, 4>());
-      else f(float(), std::integral_constant<int, 1>());
-      break;
-    case kF16:
-      if (vec && cols % 8 == 0) f(__half(), std::integral_constant<int, 8>());
-      else f(__half(), std::integral_constant<int, 1>());
-      break;
-    default:
-      if (vec && cols % 8 == 0) f(__nv_bfloat16(), std::integral_constant<int, 8>());
-      else f(__nv_bfloat16(), std::integral_constant<int, 1>());
+    case kF64: return by_pieces<double>(cols, grain, f);
+    case kF32: return by_pieces<float>(cols, grain, f);
+    case kF16: return by_pieces<__half>(cols, grain, f);
+    default: return by_pieces<__nv_bfloat16>(cols, grain, f);
   }
 }
 
@@ -289,11 +292,11 @@ int launch_dispatch(const RoutesView& r, const DenseView& x, const void* w, cons
                     cudaStream_t s) {
   if (r.tokens == 0 || x.cols == 0 || y.rows == 0) return 0;
   const int b = bytes_of(x.type);
-  by_type(x.type, x.cols, wide(x, b) && wide(y, b), [&](auto t, auto n) {
+  by_type(x.type, x.cols, std::min(grain(x, b), grain(y, b)), [&](auto t, auto n) {
     using T = decltype(t);
     constexpr int N = decltype(n)::value;
-    const Shape sh = shape_for(r, (int)(x.cols / N), dispatch_pieces(N));
-    launch(nullptr, dispatch_kernel<T, N>, grid_for(sh, sh.lanes * dispatch_pieces(N)), kThreads, 0, s, 1, sh,
+    const Shape sh = shape_for(r, (int)(x.cols / N), dispatch_pieces(N * sizeof(T)));
+    launch(nullptr, dispatch_kernel<T, N>, grid_for(sh, sh.lanes * dispatch_pieces(N * sizeof(T))), kThreads, 0, s, 1, sh,
            (const T*)x.data, x.ld, (const typename Value<T>::Acc*)w, (T*)y.data, y.ld, y.rows);
   });
   return 1;
@@ -303,11 +306,11 @@ int launch_combine(const RoutesView& r, const DenseView& h, const void* w, const
                    cudaStream_t s) {
   if (r.tokens == 0 || y.cols == 0) return 0;
   const int b = bytes_of(h.type);
-  by_type(h.type, h.cols, wide(h, b) && wide(y, b), [&](auto t, auto n) {
+  by_type(h.type, h.cols, std::min(grain(h, b), grain(y, b)), [&](auto t, auto n) {
     using T = decltype(t);
     constexpr int N = decltype(n)::value;
-    const Shape sh = shape_for(r, (int)(h.cols / N), combine_pieces(N));
-    launch(nullptr, combine_kernel<T, N>, grid_for(sh, sh.lanes * combine_pieces(N)), kThreads, 0, s, 1, sh,
+    const Shape sh = shape_for(r, (int)(h.cols / N), combine_pieces(N * sizeof(T)));
+    launch(nullptr, combine_kernel<T, N>, grid_for(sh, sh.lanes * combine_pieces(N * sizeof(T))), kThreads, 0, s, 1, sh,
            (const T*)h.data, h.ld, h.rows, (const typename Value<T>::Acc*)w, (T*)y.data, y.ld);
   });
   return 1;
@@ -317,12 +320,12 @@ int launch_combine_grad(const RoutesView& r, const DenseView& dy, const DenseVie
                         const DenseView* dh, void* dw, cudaStream_t s) {
   if (r.tokens == 0 || (dy.cols == 0 && !dw)) return 0;
   const int b = bytes_of(dy.type);
-  const bool vec = wide(dy, b) && (!h || wide(*h, b)) && (!dh || wide(*dh, b));
-  by_type(dy.type, dy.cols, vec, [&](auto t, auto n) {
+  const int g = std::min({grain(dy, b), h ? grain(*h, b) : 16, dh ? grain(*dh, b) : 16});
+  by_type(dy.type, dy.cols, g, [&](auto t, auto n) {
     using T = decltype(t);
     using A = typename Value<T>::Acc;
     constexpr int N = decltype(n)::value;
-    const Shape sh = shape_for(r, (int)(dy.cols / N), combine_pieces(N));
+    const Shape sh = shape_for(r, (int)(dy.cols / N), combine_pieces(N * sizeof(T)));
     const int per = kThreads / sh.lanes;
     launch(nullptr, combine_grad_kernel<T, N>, (r.tokens + per - 1) / per, kThreads, 0, s, 1, sh,
            (const T*)dy.data, dy.ld, h ? (const T*)h->data : nullptr, h ? h->ld : 0,

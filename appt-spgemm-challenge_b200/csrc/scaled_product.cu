@@ -113,6 +113,7 @@ __device__ __noinline__ void store_boxes(T* y, long long ldy, bool vec, const ch
   };
   if (vec) {
     const int j = lane % kPieces, left = cols - j * kPer;
+#pragma unroll 4
     for (int r = lane / kPieces; r < rows; r += 32 / kPieces) {
       T* to = y + r * ldy + j * kPer;
       if (left >= kPer) *(uint4*)to = *(const uint4*)piece(r, j);
@@ -120,8 +121,10 @@ __device__ __noinline__ void store_boxes(T* y, long long ldy, bool vec, const ch
         for (int i = 0; i < left; ++i) to[i] = piece(r, j)[i];
     }
   } else {
-    for (int r = 0; r < rows; ++r)
-      for (int c = lane; c < cols; c += 32) y[r * ldy + c] = piece(r, c / kPer)[c % kPer];
+    for (int c = lane; c < cols; c += 32) {
+#pragma unroll 8
+      for (int r = 0; r < rows; ++r) y[r * ldy + c] = piece(r, c / kPer)[c % kPer];
+    }
   }
 }
 

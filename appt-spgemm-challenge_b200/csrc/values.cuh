@@ -29,22 +29,21 @@ template <> struct Value<__nv_bfloat16> {
   static __device__ __forceinline__ __nv_bfloat16 down(float x) { return __float2bfloat16_rn(x); }
 };
 
-// N consecutive elements moved as one access: one element, or 16 bytes kept as words (arrays of
-// 16-bit elements would take a register each).
+// N consecutive elements moved as one access: one element, or 4, 8 or 16 bytes kept as words
+// (arrays of 16-bit elements would take a register each).
 template <typename T, int N>
-struct Pack {
+struct alignas(sizeof(T) * N) Pack {
   using A = typename Value<T>::Acc;
-  static constexpr int kPerWord = 4 / sizeof(T);
-  uint4 w;
+  static constexpr int kWords = sizeof(T) * N / 4;
+  unsigned word[kWords];
   __device__ __forceinline__ void up(A (&v)[N]) const {
-    static_assert(sizeof(T) * N == 16, "");
-    const unsigned word[4] = {w.x, w.y, w.z, w.w};
     if constexpr (sizeof(T) == 8) {
-      v[0] = __hiloint2double((int)w.y, (int)w.x);
-      v[1] = __hiloint2double((int)w.w, (int)w.z);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        v[i] = __hiloint2double((int)word[2 * i + 1], (int)word[2 * i]);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kWords; ++i) {
         if constexpr (sizeof(T) == 4) {
           v[i] = __uint_as_float(word[i]);
         } else if constexpr (std::is_same<T, __half>::value) {
@@ -59,13 +58,15 @@ struct Pack {
     }
   }
   __device__ __forceinline__ void down(const A (&v)[N]) {
-    unsigned word[4];
     if constexpr (sizeof(T) == 8) {
-      word[0] = (unsigned)__double2loint(v[0]), word[1] = (unsigned)__double2hiint(v[0]);
-      word[2] = (unsigned)__double2loint(v[1]), word[3] = (unsigned)__double2hiint(v[1]);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        word[2 * i] = (unsigned)__double2loint(v[i]);
+        word[2 * i + 1] = (unsigned)__double2hiint(v[i]);
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kWords; ++i) {
         if constexpr (sizeof(T) == 4) {
           word[i] = __float_as_uint(v[i]);
         } else if constexpr (std::is_same<T, __half>::value) {
@@ -77,7 +78,6 @@ struct Pack {
         }
       }
     }
-    w = make_uint4(word[0], word[1], word[2], word[3]);
   }
 };
 template <typename T>
