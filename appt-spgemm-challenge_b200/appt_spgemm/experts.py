@@ -53,6 +53,7 @@ class BlocksArg(ct.Structure):
 
 
 _ready = None
+_seen: dict = {}   # names of the dtypes seen
 
 
 def _lib() -> ct.CDLL:
@@ -105,16 +106,20 @@ class Dense:
         if isinstance(t, Dense):
             return t
         try:
-            dtype = str(t.dtype).split(".")[-1]
-            kind, where = t.device.type, t.device.index
-            ptr, shape, stride = t.data_ptr(), tuple(t.shape), tuple(t.stride())
+            dtype, where = t.dtype, t.device
+            d = Dense.__new__(Dense)
+            d.ptr, d.shape, d.strides = t.data_ptr(), tuple(t.shape), t.stride()
+            kind, d.device = where.type, where.index or 0
         except (AttributeError, TypeError):
             raise ApptError(f"{name}: needs a tensor on a CUDA device or a Dense") from None
         if kind != "cuda":
             raise ApptError(f"{name} is not on a CUDA device")
-        if dtype not in _DTYPES:
-            raise ApptError(f"{name}: type {dtype} is not supported")
-        return Dense(ptr, shape, _DTYPES[dtype], stride, where or 0)
+        if dtype not in _seen:
+            _seen[dtype] = str(dtype).split(".")[-1]
+        d.type = _DTYPES.get(_seen[dtype])
+        if d.type is None:
+            raise ApptError(f"{name}: type {_seen[dtype]} is not supported")
+        return d
 
 
 class _Call:

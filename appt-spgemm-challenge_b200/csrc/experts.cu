@@ -402,6 +402,7 @@ int appt_scaled_product(const appt_scaled* A, const appt_blocks* W, const int32_
       refuse("W: data must be aligned to 16 bytes, scale to 4, neither null");
     if (a.q.cols != w.cols) refuse("A and W differ in columns");
     if (a.q.ld % 16) refuse("A: ld must be a multiple of 16");
+    if (a.q.rows > 1 << 30 || w.rows > 1 << 30) refuse("more than 2^30 rows of A or W");
     const DenseView y = view(Y, "Y", kShortTypes);
     if (y.rows != a.q.rows || y.cols != w.rows) refuse("Y must be A's rows x W's rows");
     if (!group_ptr && w.groups != 1) refuse("group_ptr may be null with one group only");

@@ -259,7 +259,7 @@ Shape shape_for(const RoutesView& r, int pieces, int each) {
 dim3 grid_for(const Shape& s, long long per_cta_pieces) {
   const int per = kThreads / s.lanes;
   const long long y = ((long long)s.pieces + per_cta_pieces - 1) / per_cta_pieces;
-  return dim3((s.tokens + per - 1) / per, (unsigned)(y > 65535 ? 65535 : y));
+  return dim3((unsigned)(((long long)s.tokens + per - 1) / per), (unsigned)(y > 65535 ? 65535 : y));
 }
 
 template <typename T, typename F>
@@ -327,7 +327,7 @@ int launch_combine_grad(const RoutesView& r, const DenseView& dy, const DenseVie
     constexpr int N = decltype(n)::value;
     const Shape sh = shape_for(r, (int)(dy.cols / N), combine_pieces(N * sizeof(T)));
     const int per = kThreads / sh.lanes;
-    launch(nullptr, combine_grad_kernel<T, N>, (r.tokens + per - 1) / per, kThreads, 0, s, 1, sh,
+    launch(nullptr, combine_grad_kernel<T, N>, (unsigned)((r.tokens + per - 1ll) / per), kThreads, 0, s, 1, sh,
            (const T*)dy.data, dy.ld, h ? (const T*)h->data : nullptr, h ? h->ld : 0,
            h ? h->rows : dh->rows, (const A*)w, dh ? (T*)dh->data : nullptr, dh ? dh->ld : 0,
            (A*)dw);

@@ -45,6 +45,7 @@ constexpr int kMaxStages = 10;
 constexpr int kMaxBuffers = 4;
 constexpr int kSharedMax = 227 * 1024;
 constexpr int kOutBox = 32 * 128;
+constexpr int kRegsFew = 72, kRegsMany = 216;   // see Shape::kMoveRegs
 
 struct Params {
   const float* sa;
@@ -287,7 +288,7 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
   const int kb1 = (int)((long long)p.k_blocks * (rank + 1) / splits);
 
   if (warp < 4) {
-    if (S::kMoveRegs) regs_fewer<72>();
+    if (S::kMoveRegs) regs_fewer<kRegsFew>();
     if (warp == 0) {
       // ---- tiles by TMA
       int it = 0, st = 0;
@@ -369,7 +370,7 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
     __syncwarp();
   } else {
     // ---- scaling, adding, writing
-    if (S::kMoveRegs) regs_more<216>();
+    if (S::kMoveRegs) regs_more<kRegsMany>();
     const int wg = (warp - 4) / 4, quarter = warp & 3;
     const int who = quarter * 32 + lane;         // lane of the tile
     const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16) + wg * kPart;
@@ -568,6 +569,18 @@ void product(const ScaledView& a, const BlocksView& w, const Params& p, int sms,
   static_assert(S::kStages >= 3, "");
   static_assert(!kSwap || kCols * kLanes * 4 <= S::kStages * S::kStageBytes, "");
   static std::atomic<unsigned long long> opted{0};
+  if (S::kMoveRegs) {
+    // a kernel built to fewer registers could never hand the adding warps theirs: they would wait
+    static std::atomic<int> regs{0};
+    if (regs.load() == 0) {
+      cudaFuncAttributes fa = {};
+      const cudaError_t e = cudaFuncGetAttributes(&fa, product_kernel<kSwap, kCols>);
+      if (e != cudaSuccess) throw LaunchFailed{e};
+      regs.store(fa.numRegs);
+    }
+    if (regs.load() * S::kThreads < 128 * kRegsFew + 256 * kRegsMany)
+      throw LaunchFailed{cudaErrorLaunchOutOfResources};
+  }
   const CUtensorMap ma = map_of(a.q.data, a.q.cols, a.q.rows, a.q.ld, 1, 0, S::kRowTile, 2);
   const CUtensorMap mw =
       map_of(w.data, w.cols, w.rows, w.ld, w.groups, w.group_stride, S::kNTile, 3);

@@ -402,7 +402,8 @@ int appt_dispatch_quantize(const appt_routes *routes, const appt_dense *X, const
  * 1] - 1 (groups + 1 device entries, ascending, e.g. expert_ptr; NULL with one group: all rows).
  * Rows of no group are left as they were. Y: F32, F16 or BF16, rows x W.rows; sums in F32,
  * rounded once. A.q.ld must be a multiple of 16 and A.q.data 16-byte aligned; any number of
- * columns. */
+ * columns, up to 2^30 rows of A and of W. The product of a row's and a block's scale is formed in
+ * F32 and must not overflow there. */
 int appt_scaled_product(const appt_scaled *A, const appt_blocks *W, const int32_t *group_ptr,
                         const appt_dense *Y, int32_t device, void *stream);
 /* Waits for `device` and returns APPT_ERR_DEVICE when a product on it has given up one of its

@@ -728,6 +728,49 @@ def test_layer_of_experts_captured_and_replayed():
             check_layer(t, experts)
 
 
+def test_route_captured_and_replayed():
+    """A route of two kernels, the second of which starts before the first has ended, replayed on new
+    ids, back to back and each time after a kernel that writes them."""
+    tokens, top_k, experts = 9000, 4, 200
+    ids = torch.zeros(tokens, top_k, dtype=torch.int32, device=DEV)
+    call, *out = route(ids, experts)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call.run(stream())
+        call.run(stream())
+    for seed in range(4):
+        ids.copy_(ids_for(gen(seed), tokens, top_k, experts, "wild"))
+        out[1].fill_(-7)
+        graph.replay()
+        check_route(ids, experts, *out)
+
+
+def test_a_call_in_another_thread_and_on_the_default_stream():
+    """Calls are made from the thread that has the data; errors are a thread's own."""
+    import threading
+    t, calls = layer(40, 2, 8, 256, 128)
+    new_inputs(t, 8, 70)
+    torch.cuda.synchronize()
+    failed = []
+
+    def work():
+        try:
+            for c in calls:
+                c.run()
+            with pytest.raises(ap.ApptError):
+                ex.Dispatch(ex.Routes(1, 1, ex.Dense(0, (1,), "i32")), t["x"][:1], t["y"][:1]).run()
+        except BaseException as e:   # for the test's own thread
+            failed.append(e)
+
+    th = threading.Thread(target=work)
+    th.start()
+    th.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    check_layer(t, 8)
+
+
 def test_layers_on_two_streams_and_equal_bits():
     """Two layers at once on streams of their own, a side stream's work ordered by the stream
     alone; the same inputs again give the same bits."""
