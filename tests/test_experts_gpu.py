@@ -728,6 +728,32 @@ def test_layer_of_experts_captured_and_replayed():
             check_layer(t, experts)
 
 
+FIRST_IN_A_CAPTURE = """
+import sys
+sys.path[:0] = {paths!r}
+import torch
+import test_experts_gpu as t
+for case in ((24, 4, 16, 256, 128), (3000, 8, 8, 384, 256)):
+    made, calls = t.layer(*case)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for c in calls:
+            c.run(t.stream())
+    t.new_inputs(made, case[2], 40)
+    graph.replay()
+    t.check_layer(made, case[2])
+print("ok")
+"""
+
+
+def test_a_process_s_first_calls_are_captured():
+    """Nothing is set up by a first call outside of a capture."""
+    code = FIRST_IN_A_CAPTURE.format(paths=[str(Path(__file__).parent), *map(str, sys.path)])
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "ok" in r.stdout, r.stderr[-2000:]
+
+
 def test_route_captured_and_replayed():
     """A route of two kernels, the second of which starts before the first has ended, replayed on new
     ids, back to back and each time after a kernel that writes them."""
