@@ -406,9 +406,10 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
         pa = p.sa + min(t.row + who, t.row_end - 1);
         pw = p.sw + ((long long)t.group * p.n_blocks +
                      min((t.n + wg * kPart) / kScaleBlock, p.n_blocks - 1)) * p.k_blocks;
-        const int second = min(1, p.k_blocks - 1);
+        const int second = min(1, p.k_blocks - 1), third = min(2, p.k_blocks - 1);
         a0 = pa[0], w0 = pw[0];
         a1 = pa[second * p.sa_ld], w1 = pw[second];
+        pa += third * p.sa_ld, pw += third;   // the next block's but one, or the last again
       };
       // Adds one partial tile, kChunk columns at a time, and hands its buffer back as soon as the
       // last of them is in registers.
@@ -419,12 +420,14 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
         if (!ok) return;
         fence_after();
         const uint64_t scale = two(a * w, a * w);
-        const int then = min(kb + 2, p.k_blocks - 1);
 #pragma unroll
         for (int c = 0; c < kPart; c += kChunk) {
           uint32_t now[kChunk];
           tmem_load(now, buffer(it) + c);
-          if (c == 0) a = pa[then * p.sa_ld], w = pw[then];
+          if (c == 0) {
+            a = *pa, w = *pw;
+            if (kb + 3 < p.k_blocks) pa += p.sa_ld, ++pw;
+          }
           tmem_wait(now);
           if (c + kChunk == kPart) buffer_read(it);
 #pragma unroll
