@@ -64,6 +64,9 @@ struct Params {
   void* y;
   long long ldy;
   int rows, n, k_blocks, n_blocks, groups, type;
+  int n_tiles;               // tiles of a row of tiles
+  int step_rows, step_cols;  // from a CTA's tile to its next
+  int splits_log2;           // CTAs that share a tile's K
   bool vec;            // rows of y start on 16 bytes
 };
 
@@ -96,7 +99,8 @@ struct Shape {
   static constexpr int kPart = kCols / kGroups;                // columns of a warpgroup
   // Y on its way out: a warp's boxes of 32 rows x 128 bytes, enough for its 16-bit values
   static constexpr int kOutBoxes = kPart / 64;
-  static constexpr int kOutBytes = kSwap ? 0 : 4 * kGroups * kOutBoxes * kOutBox;
+  static constexpr int kOutBytes =
+      kSwap ? kCols * kLanes * 4 : 4 * kGroups * kOutBoxes * kOutBox;
   static constexpr int kFixedBytes = kOutBytes + (int)sizeof(Groups) + (int)sizeof(Barriers) + 64 +
                                      kScaleStages * kScaleFloats * 4 + 1024;
   static constexpr int kStages = (kSharedMax - kFixedBytes) / kStageBytes < kMaxStages
@@ -183,8 +187,17 @@ __device__ __forceinline__ void write_rows(const Params& p, const CUtensorMap* m
 // groups never overlap and never leave the operands, whatever the offsets are.
 template <int kRowTile>
 __device__ void fill_groups(const Params& p, Groups* t) {
+  if (!p.group_ptr) {
+    if (threadIdx.x == 0) {
+      t->row[0] = t->tile[0] = 0;
+      t->row[1] = p.rows;
+      t->tile[1] = (p.rows + kRowTile - 1) / kRowTile;
+    }
+    __syncthreads();
+    return;
+  }
   for (int g = threadIdx.x; g <= p.groups; g += blockDim.x)
-    t->row[g] = p.group_ptr ? min(max(p.group_ptr[g], 0), p.rows) : (g ? p.rows : 0);
+    t->row[g] = min(max(p.group_ptr[g], 0), p.rows);
   __syncthreads();
   if (threadIdx.x < 32) {
     int most = 0, tiles = 0;
@@ -221,24 +234,21 @@ struct Tile {
 template <int kRowTile, int kNTile>
 struct Tiles {
   const Groups* t;
-  int tiles, n_tiles, i, step, step_rows, step_cols, row, col, group;
-  __device__ __forceinline__ Tiles(const Groups* groups, int tiles_, int n_tiles_, int first,
-                                   int step_)
-      : t(groups), tiles(tiles_), n_tiles(n_tiles_), i(first), step(step_) {
-    step_rows = step / n_tiles;
-    step_cols = step - step_rows * n_tiles;
+  int rows, n_tiles, step_rows, step_cols, row, col, group;
+  __device__ __forceinline__ Tiles(const Params& p, const Groups* groups, int i)
+      : t(groups), rows(groups->tile[p.groups]), n_tiles(p.n_tiles), step_rows(p.step_rows),
+        step_cols(p.step_cols) {
     row = i / n_tiles;
     col = i - row * n_tiles;
     group = 0;
   }
-  __device__ __forceinline__ bool more() const { return i < tiles; }
+  __device__ __forceinline__ bool more() const { return row < rows; }
   __device__ __forceinline__ Tile at() {
     while (t->tile[group + 1] <= row) ++group;   // ends: row is below the last entry
     return Tile{group, t->row[group] + (row - t->tile[group]) * kRowTile, t->row[group + 1],
                 col * kNTile};
   }
   __device__ __forceinline__ void next() {
-    i += step;
     row += step_rows;
     col += step_cols;
     if (col >= n_tiles) col -= n_tiles, ++row;
@@ -249,12 +259,13 @@ template <bool kSwap, int kCols>
 __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_a,
                    const __grid_constant__ CUtensorMap map_w,
-                   const __grid_constant__ CUtensorMap map_y, const Params p, int splits) {
+                   const __grid_constant__ CUtensorMap map_y, const Params p) {
   using S = Shape<kSwap, kCols>;
   constexpr int kPart = S::kPart;             // columns of a warpgroup
   extern __shared__ char raw[];
   char* base = (char*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
   char* out = base + S::kStages * S::kStageBytes;   // on 1024 bytes, as the swizzle wants it
+  float* shares = (float*)out;                      // partial sums of a tile whose K is split
   Groups* groups = (Groups*)(out + S::kOutBytes);
   float* scales = (float*)(groups + 1);
   Barriers* bars = (Barriers*)(((uintptr_t)(scales + kScaleStages * S::kScaleFloats) + 7) &
@@ -263,24 +274,26 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
   volatile int* gave_up = (volatile int*)(tmem_slot + 1);
 
   const int warp = __shfl_sync(kFull, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < S::kStages; ++i) {
-      mbar_init(smem_u32(&bars->full[i]), 1);
-      mbar_init(smem_u32(&bars->empty[i]), 1);
+  if (warp == 0) {
+    if (lane < S::kStages) {
+      mbar_init(smem_u32(&bars->full[lane]), 1);
+      mbar_init(smem_u32(&bars->empty[lane]), 1);
     }
-    for (int i = 0; i < S::kBuffers; ++i) {
-      mbar_init(smem_u32(&bars->tfull[i]), 1);
-      mbar_init(smem_u32(&bars->tempty[i]), 4 * S::kGroups);
+    if (lane < S::kBuffers) {
+      mbar_init(smem_u32(&bars->tfull[lane]), 1);
+      mbar_init(smem_u32(&bars->tempty[lane]), 4 * S::kGroups);
     }
-    for (int i = 0; i < kScaleStages; ++i) {
-      mbar_init(smem_u32(&bars->sfull[i]), 64);
-      mbar_init(smem_u32(&bars->sempty[i]), 8);
+    if (lane < kScaleStages) {
+      mbar_init(smem_u32(&bars->sfull[lane]), 64);
+      mbar_init(smem_u32(&bars->sempty[lane]), 8);
     }
-    mbar_init(smem_u32(&bars->drain), 1);
+    if (lane == 0) {
+      mbar_init(smem_u32(&bars->drain), 1);
+      *gave_up = 0;
+      tma_prefetch_map(&map_a);
+      tma_prefetch_map(&map_w);
+    }
     mbar_init_fence();
-    *gave_up = 0;
-    tma_prefetch_map(&map_a);
-    tma_prefetch_map(&map_w);
   }
   if (warp == 1) tmem_alloc(smem_u32(tmem_slot), S::kTmemColumns);
   fence_before();
@@ -288,13 +301,14 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
   fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  const int n_tiles = (p.n + S::kNTile - 1) / S::kNTile;
-  const int tiles = groups->tile[p.groups] * n_tiles;   // below 2^31: checked by the host
-  const int rank = splits > 1 ? (int)cluster_rank() : 0;
-  const int first = blockIdx.x / splits, step = gridDim.x / splits;
-  Tiles<S::kRowTile, S::kNTile> order(groups, tiles, n_tiles, first, step);
-  const int kb0 = (int)((long long)p.k_blocks * rank / splits);
-  const int kb1 = (int)((long long)p.k_blocks * (rank + 1) / splits);
+  const int splits = 1 << p.splits_log2;
+  const int rank = kSwap && splits > 1 ? (int)cluster_rank() : 0;
+  // Every thread arrives here and waits once: warps that write to the other CTAs' shared memory
+  // before they do (the CTAs run by then), the others at the end of their roles.
+  if (kSwap && splits > 1) cluster_arrive();
+  Tiles<S::kRowTile, S::kNTile> order(p, groups, blockIdx.x >> p.splits_log2);
+  const int kb0 = p.k_blocks * rank >> p.splits_log2;   // k_blocks < 2^24
+  const int kb1 = p.k_blocks * (rank + 1) >> p.splits_log2;
 
   if (warp < 4) {
     if (S::kMoveRegs) regs_fewer<kRegsFew>();
@@ -377,6 +391,7 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
       cp_async_wait_all();
     }
     __syncwarp();
+    if (kSwap && splits > 1) cluster_wait();
   } else {
     // ---- scaling, adding, writing
     if (S::kMoveRegs) regs_more<kRegsMany>();
@@ -460,6 +475,7 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
       }
       bulk_wait();
     } else {
+      bool waited = false;
       for (; order.more(); order.next()) {
         const Tile t = order.at();
         clear();
@@ -489,10 +505,18 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
 #pragma unroll
         for (int c = 0; c < kPart; c += 2) untwo(pairs[c / 2], sum[c], sum[c + 1]);
         if (splits > 1) {
-          // the stages are free: every load has been used by a product that is done
-          float* part = (float*)base;
+          // every rank gets its share of the columns from all: c % splits == rank
+          cluster_wait();
+          waited = true;
 #pragma unroll
-          for (int c = 0; c < kPart; ++c) part[(wg * kPart + c) * kLanes + who] = sum[c];
+          for (int c = 0; c < kPart; ++c) {
+            const int col = wg * kPart + c;
+            if (t.row + col < t.row_end)
+              store_cluster(map_shared(smem_u32(shares + ((rank * kCols + col) >> p.splits_log2) *
+                                                             kLanes + who),
+                                       col & (splits - 1)),
+                            sum[c]);
+          }
         } else if (t.n + who < p.n) {
 #pragma unroll
           for (int c = 0; c < kPart; ++c) {
@@ -501,26 +525,26 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
           }
         }
       }
+      if (splits > 1 && !waited) cluster_wait();
     }
     if (!ok && lane == 0) g_product_gave_up = 1;
   }
   if constexpr (kSwap) {
     if (splits > 1) {
-      // one tile per cluster: every CTA adds its share of the columns over all ranks
+      // one tile per cluster: every CTA adds its share of the columns over all ranks, in their order
       cluster_sync();
-      if (first < tiles && warp >= 4) {
-        const Tile t = Tiles<S::kRowTile, S::kNTile>(groups, tiles, n_tiles, first, step).at();
+      Tiles<S::kRowTile, S::kNTile> mine(p, groups, blockIdx.x >> p.splits_log2);
+      if (mine.more() && warp >= 4) {
+        const Tile t = mine.at();
         const int who = threadIdx.x & (kLanes - 1), wg = (warp - 4) / 4;
-        for (int c = rank + splits * wg; c < kCols; c += 2 * splits) {
-          const int r = t.row + c;
-          if (r >= t.row_end || t.n + who >= p.n) continue;
-          const uint32_t at = smem_u32((float*)base + c * kLanes + who);
-          float v = 0.f;
-          for (int q = 0; q < splits; ++q) v += load_cluster(map_shared(at, q));
-          store_one(p, r * p.ldy + t.n + who, v);
+        const int each = kCols >> p.splits_log2;
+        const int last = t.n + who < p.n ? t.row_end - t.row : 0;
+        for (int i = wg; i < each && i * splits + rank < last; i += 2) {
+          float sum = 0.f;
+          for (int q = 0; q < splits; ++q) sum += shares[(q * each + i) * kLanes + who];
+          store_one(p, (t.row + i * splits + rank) * p.ldy + t.n + who, sum);
         }
       }
-      cluster_sync();   // no CTA leaves while another reads its part
     }
   }
   fence_before();
@@ -576,10 +600,9 @@ long long row_tiles_for(long long rows, long long groups, int tile) {
 }
 
 template <bool kSwap, int kCols>
-void product(const ScaledView& a, const BlocksView& w, const Params& p, int sms, cudaStream_t s) {
+void product(const ScaledView& a, const BlocksView& w, Params p, int sms, cudaStream_t s) {
   using S = Shape<kSwap, kCols>;
   static_assert(S::kStages >= 3, "");
-  static_assert(!kSwap || kCols * kLanes * 4 <= S::kStages * S::kStageBytes, "");
   static std::atomic<unsigned long long> opted{0};
   if (S::kMoveRegs) {
     // a kernel built to fewer registers could never hand the adding warps theirs: they would wait
@@ -604,14 +627,18 @@ void product(const ScaledView& a, const BlocksView& w, const Params& p, int sms,
   const long long n_tiles = (p.n + S::kNTile - 1) / S::kNTile;
   const long long tiles = row_tiles_for(p.rows, p.groups, S::kRowTile) * n_tiles;
   if (tiles > INT_MAX - sms) throw LaunchFailed{cudaErrorInvalidValue};   // no memory holds such a Y
-  int splits = 1;
+  int log2 = 0;
   if (kSwap)
     // (a cluster's CTAs share a GPC, whose SMs the clusters may not all fill: a second wave of
     // them took 13.7 us where 7 was expected)
-    while (splits < 8 && tiles * splits * 2 <= sms * 7 / 8 && splits * 2 <= p.k_blocks) splits *= 2;
-  const long long ctas = splits > 1 ? tiles * splits : tiles < sms ? tiles : sms;
-  launch(&opted, product_kernel<kSwap, kCols>, dim3((unsigned)ctas), dim3(S::kThreads), S::kBytes, s,
-         splits, ma, mw, my, p, splits);
+    while (log2 < 3 && tiles << (log2 + 1) <= sms * 7 / 8 && 2 << log2 <= p.k_blocks) ++log2;
+  const long long step = log2 || tiles < sms ? tiles : sms;
+  p.n_tiles = (int)n_tiles;
+  p.step_rows = (int)(step / n_tiles);
+  p.step_cols = (int)(step % n_tiles);
+  p.splits_log2 = log2;
+  launch(&opted, product_kernel<kSwap, kCols>, dim3((unsigned)(step << log2)), dim3(S::kThreads),
+         S::kBytes, s, 1 << log2, ma, mw, my, p);
 }
 
 }  // namespace

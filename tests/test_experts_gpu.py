@@ -439,7 +439,9 @@ def test_quantize_gated(shape, dtype):
     n = max(0, min(used, rows))
     gate, up = x[:n, :width].double(), x[:n, width:].double()
     v = gate * torch.sigmoid(gate) * up
-    # exp to 2 ulp, then a sum, a quotient and a product of half a step each: below 8 half steps
+    # 2^x to 2 ulp and its argument's rounding (|g| half steps, of which the 1 in 1 + exp(-g) leaves
+    # less than 1.3 where |silu| is largest), a reciprocal to 1 ulp, a sum and two products of half a
+    # step each: below 10 half steps
     amax = blocked(v).abs().amax(-1)
     close(scale[:, :n].t(), (amax / 448).clamp(min=torch.finfo(F32).tiny), 10 * u(F32) * amax / 448)
     step = scale[:, :n].t().double().repeat_interleave(128, 1)[:, :width]
