@@ -18,18 +18,18 @@
 // are the lanes and the rows the columns (16 to 64 of them): a tile of 128 rows would be mostly
 // padding, and the tensor cores' time goes by the columns. A row's scale is then one per column,
 // read from shared memory.
-// With fewer tiles than half the SMs, a cluster of CTAs splits a tile along K and adds its parts
-// through distributed shared memory in the order of the ranks, so the result does not depend on
-// timing.
+// With fewer tiles than half the SMs, a cluster of CTAs splits a tile along K. Each CTA sends its
+// sums through distributed shared memory to the columns' owners, which add them in the order of
+// the ranks, so the result does not depend on timing.
 //
 // Many rows: bound by the scaling and adding, not by the tensor cores. A block of 128 x 256 takes
 // them 512 cycles and the adding warps some 820: 256 for its fused multiply-adds, about as much for
 // the reads of tensor memory between them, the rest for waiting on one buffer and handing back the
 // other. Neither more adding warps (4 warpgroups of 64 columns), nor pairs of CTAs on tiles of 256
 // rows (a third less traffic from L2), nor halves of 128 columns with barriers of their own were
-// faster. 8192 x 8192 x 4096 takes 262 us, 2.1 PFLOP/s (307 us at the clocks that 1000 W leave it),
-// 32,768 sorted rows x 2048 x 2048 over 64 groups 176 us. Few rows: bound by the weights' bytes;
-// 128 rows over 56 of 64 groups, 4096 x 2048, 79 us, 6.0 TB/s; one row x 4096 x 4096 6.9 us.
+// faster. 8192 x 8192 x 4096 takes 259 us, 2.1 PFLOP/s (300 us at the clocks that 1000 W leave it),
+// 32,768 sorted rows x 2048 x 2048 over 64 groups 174 us. Few rows: bound by the weights' bytes;
+// 128 rows over 56 of 64 groups, 4096 x 2048, 78 us, 6.1 TB/s; one row x 4096 x 4096 6.2 us.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <climits>
