@@ -202,7 +202,7 @@ class _Call:
 
 class Routes:
     """Where Route put each pair: pair_row has an int32 entry for each of the tokens * top_k
-    pairs, its sorted row, -1 for a dropped pair."""
+    pairs, its sorted row, -1 for a dropped pair. No two kept pairs have the same row."""
 
     def __init__(self, tokens: int, top_k: int, pair_row):
         self.tokens, self.top_k, self.pair_row = int(tokens), int(top_k), pair_row
@@ -281,7 +281,8 @@ class CombineGrad(_Call):
 
 class Quantize(_Call):
     """Rows of x to e4m3 with an f32 scale for each row and block of 128 columns: scale
-    [ceil(cols / 128), rows], q [rows, cols]. gate "silu": the values are silu(x[:, :n]) * x[:, n:].
+    [ceil(cols / 128), rows], q [rows, cols]. gate "silu": the values are silu(x[:, :n]) * x[:, n:],
+    silu taken as 0 below -87.
     rows_ptr (one i32 on the device): only that many rows are read and written."""
 
     def __init__(self, x, q, scale, rows_ptr=None, gate: str | None = None):

@@ -76,6 +76,9 @@ bool overlap(const Span& a, const Span& b) {
   return true;
 }
 
+// Bytes that an operand may span: well above any memory, and no address arithmetic wraps below.
+constexpr long long kLargest = 1ll << 50;
+
 const DenseView view(const appt_dense* m, const char* name, unsigned types, int align = 0) {
   if (!m) refuse(std::string(name) + " is null");
   const int b = m->type < 0 || m->type > kI64 || !(types >> m->type & 1) ? 0 : type_bytes(m->type);
@@ -90,6 +93,8 @@ const DenseView view(const appt_dense* m, const char* name, unsigned types, int 
   v.ld = m->rows > 1 ? m->ld : (m->cols + 15) / 16 * 16;
   if (m->rows > 1 && (m->ld < m->cols || m->ld >= INT_MAX))
     refuse(std::string(name) + ": ld must be at least cols and below 2^31 - 1");
+  if (v.ld > 0 && v.rows > kLargest / 8 / v.ld)
+    refuse(std::string(name) + ": its rows reach further than any memory");
   v.data = m->data;
   if (v.rows > 0 && v.cols > 0) {
     if (!v.data) refuse(std::string(name) + ": null data");
@@ -394,6 +399,7 @@ int appt_scaled_product(const appt_scaled* A, const appt_blocks* W, const int32_
     w.ld = w.rows > 1 ? W->ld : (w.cols + 15) / 16 * 16;
     if (w.ld < w.cols || w.ld % 16 || w.ld >= (1ll << 38))
       refuse("W: ld must be a multiple of 16 and at least cols");
+    if (w.rows > kLargest / w.ld) refuse("W: its rows reach further than any memory");
     w.group_stride = w.groups > 1 ? W->group_stride : (w.rows - 1) * w.ld + (w.cols + 15) / 16 * 16;
     if (w.group_stride < (w.rows - 1) * w.ld + w.cols || w.group_stride % 16 ||
         w.group_stride >= (1ll << 40))

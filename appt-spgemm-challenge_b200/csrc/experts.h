@@ -18,9 +18,10 @@ struct LaunchFailed {   // thrown by launch(), turned into a status at the C ent
 // what it reads).
 constexpr int kAfterStart = 0;
 
-// kernel<<<grid, block, smem, s>>>(args...) in clusters of `cluster` CTAs, with the launch's own status (an error that an
-// earlier call of the program left behind is not taken for it). The opt-in to more than 48 KB of
-// shared memory, static and dynamic together, is per device and kept in *opted, a bit per device.
+// kernel<<<grid, block, smem, s>>>(args...) in clusters of `cluster` CTAs, with the launch's own
+// status (an error that an earlier call of the program left behind is not taken for it). The opt-in
+// to more than 48 KB of shared memory, static and dynamic together, is per device and kept in
+// *opted, a bit per device.
 constexpr size_t kStaticMost = 16 * 1024;   // of any kernel here that also has dynamic memory
 template <typename... P, typename... A>
 void launch(std::atomic<unsigned long long>* opted, void (*kernel)(P...), dim3 grid, dim3 block,

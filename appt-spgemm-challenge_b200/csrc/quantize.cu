@@ -3,9 +3,9 @@
 //   scale = max(amax / 448, smallest normal float),   q = e4m3(value / scale)
 //
 // value is X, or silu(X[:, :n]) X[:, n:]; for dispatch, a token's row is quantised once and
-// written to each of its pairs' rows. The largest magnitude of a block is
-// a maximum over its lanes that keeps a NaN. The quotients are rounded as divisions are (a
-// product with the reciprocal would round differently), at three instructions each.
+// written to each of its pairs' rows. The largest magnitude of a block is a maximum over its lanes
+// that keeps a NaN. The quotients are rounded as divisions are (a product with the reciprocal would
+// round differently), at three instructions each.
 //
 // Bound by memory, but only just: some 25 (gated) instructions per element are 70 % of what the SMs
 // can issue. Gated bf16 16384 x 2048: 30 us, 5.6 TB/s (with both operands unpacked as they arrive 37,
@@ -25,8 +25,8 @@ namespace {
 constexpr int kThreads = 256;
 
 // How a block's columns lie in its lanes. kVec: 8 lanes of 16 neighbouring columns (32 bits: 16 lanes
-// of 8, so that a lane's 16-byte words are two neighbours of another lane's), moved as such. Else (rows that do not start on 16 bytes) 32 lanes of 4 neighbouring columns, read one by
-// one, and stored as a word where rows of Q start on 4 bytes.
+// of 8), moved as 16-byte words. Else (rows that do not start on 16 bytes) 32 lanes of 4 neighbouring
+// columns, read one by one, and stored as a word where rows of Q start on 4 bytes.
 template <typename T, bool kVec>
 struct Lay {
   static constexpr int kLanes = !kVec ? 32 : sizeof(T) == 4 ? 16 : 8;

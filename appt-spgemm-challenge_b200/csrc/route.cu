@@ -5,11 +5,11 @@
 //
 // The pairs are cut into one contiguous chunk per CTA. An expert's base in chunk b is expert_ptr[e]
 // plus its counts in the chunks before b, so a CTA needs the other chunks' counts and no order
-// among CTAs. Up to 8 chunks are one cluster and read each other's counts from shared memory; more get them from a kernel that counts first (whose end the placing kernel waits for
-// only once its own counting is done). Within a chunk each warp owns a contiguous part, counts it
-// per expert in shared memory, and places 32 pairs at a time: the rank among equal ids of the 32
-// lanes is a popcount of the match mask. No atomic decides an order, so equal inputs give equal
-// outputs.
+// among CTAs. Up to 8 chunks are one cluster and read each other's counts from shared memory; more
+// get them from a kernel that counts first (whose end the placing kernel waits for only once its
+// own counting is done). Within a chunk each warp owns a contiguous part, counts it per expert in
+// shared memory, and places 32 pairs at a time: the rank among equal ids of the 32 lanes is a
+// popcount of the match mask. No atomic decides an order, so equal inputs give equal outputs.
 //
 // Bound by latency: a chain of some six barriers and two trips to memory. 256 pairs (64 experts)
 // 2.9 us, 4,096 (256 experts) 5.0 us, 524,288 (6.2 MB) 10.9 us, of which the counting kernel takes

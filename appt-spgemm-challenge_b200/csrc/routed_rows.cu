@@ -300,8 +300,9 @@ int launch_dispatch(const RoutesView& r, const DenseView& x, const void* w, cons
     using T = decltype(t);
     constexpr int N = decltype(n)::value;
     const Shape sh = shape_for(r, (int)(x.cols / N), dispatch_pieces(N * sizeof(T)));
-    launch(nullptr, dispatch_kernel<T, N>, grid_for(sh, sh.lanes * dispatch_pieces(N * sizeof(T))), kThreads, 0, s, 1, sh,
-           (const T*)x.data, x.ld, (const typename Value<T>::Acc*)w, (T*)y.data, y.ld, y.rows);
+    launch(nullptr, dispatch_kernel<T, N>, grid_for(sh, sh.lanes * dispatch_pieces(N * sizeof(T))),
+           kThreads, 0, s, 1, sh, (const T*)x.data, x.ld,
+           (const typename Value<T>::Acc*)w, (T*)y.data, y.ld, y.rows);
   });
   return 1;
 }
@@ -314,8 +315,9 @@ int launch_combine(const RoutesView& r, const DenseView& h, const void* w, const
     using T = decltype(t);
     constexpr int N = decltype(n)::value;
     const Shape sh = shape_for(r, (int)(h.cols / N), combine_pieces(N * sizeof(T)));
-    launch(nullptr, combine_kernel<T, N>, grid_for(sh, sh.lanes * combine_pieces(N * sizeof(T))), kThreads, 0, s, 1, sh,
-           (const T*)h.data, h.ld, h.rows, (const typename Value<T>::Acc*)w, (T*)y.data, y.ld);
+    launch(nullptr, combine_kernel<T, N>, grid_for(sh, sh.lanes * combine_pieces(N * sizeof(T))),
+           kThreads, 0, s, 1, sh, (const T*)h.data, h.ld, h.rows,
+           (const typename Value<T>::Acc*)w, (T*)y.data, y.ld);
   });
   return 1;
 }
@@ -331,8 +333,8 @@ int launch_combine_grad(const RoutesView& r, const DenseView& dy, const DenseVie
     constexpr int N = decltype(n)::value;
     const Shape sh = shape_for(r, (int)(dy.cols / N), combine_pieces(N * sizeof(T)));
     const int per = kThreads / sh.lanes;
-    launch(nullptr, combine_grad_kernel<T, N>, (unsigned)((r.tokens + per - 1ll) / per), kThreads, 0, s, 1, sh,
-           (const T*)dy.data, dy.ld, h ? (const T*)h->data : nullptr, h ? h->ld : 0,
+    launch(nullptr, combine_grad_kernel<T, N>, (unsigned)((r.tokens + per - 1ll) / per), kThreads,
+           0, s, 1, sh, (const T*)dy.data, dy.ld, h ? (const T*)h->data : nullptr, h ? h->ld : 0,
            h ? h->rows : dh->rows, (const A*)w, dh ? (T*)dh->data : nullptr, dh ? dh->ld : 0,
            (A*)dw);
   });

@@ -335,7 +335,9 @@ typedef struct appt_routes { /* where each pair went, as appt_route fills it */
   int32_t top_k;
   int32_t reserved;        /* 0 */
   const int32_t *pair_row; /* tokens * top_k: the pair's sorted row; a value outside the row
-                              matrix (-1) is a dropped pair, which is neither read nor written */
+                              matrix (-1) is a dropped pair, which is neither read nor written.
+                              Kept pairs have rows of their own: where two name one row, what
+                              the calls that write sorted rows leave in it is not defined */
 } appt_routes;
 
 typedef struct appt_scaled { /* values in 8 bits with one scale per row and block of 128 columns */
@@ -361,7 +363,7 @@ size_t appt_route_workspace(int64_t tokens, int32_t top_k, int64_t experts);
 /* Sorts the pairs by expert, stably. ids: tokens x top_k, APPT_I32 or APPT_I64; an id outside
  * [0, experts) drops its pair. Fills expert_ptr (experts + 1: expert e has the sorted rows
  * expert_ptr[e] .. expert_ptr[e + 1] - 1), row_pair (room for tokens * top_k; the kept rows are
- * written) and pair_row (tokens * top_k; -1 for dropped pairs). tokens * top_k < 2^31, experts
+ * written) and pair_row (tokens * top_k; -1 for dropped pairs). tokens * top_k < 2^31 - 1, experts
  * <= APPT_MAX_EXPERTS. (expert_ptr, row_pair) is the CSR form of the transposed routing. */
 int appt_route(const appt_dense *ids, int64_t experts, int32_t *expert_ptr, int32_t *row_pair,
                int32_t *pair_row, void *workspace, size_t workspace_bytes, int32_t device,
@@ -386,7 +388,8 @@ int appt_combine_grad(const appt_routes *routes, const appt_dense *dY, const app
                       void *stream);
 
 #define APPT_GATE_NONE 0
-#define APPT_GATE_SILU 1 /* values are silu(X[:, :n]) * X[:, n:], n = Q's columns, X has 2 n */
+#define APPT_GATE_SILU 1 /* values are silu(X[:, :n]) * X[:, n:], n = Q's columns, X has 2 n;
+                            silu of values below -87 is 0 */
 
 /* Rows to 8 bits: for each row and block of 128 columns, scale = max(|largest value| / 448,
  * smallest normal float), q = value / scale rounded to nearest even. A NaN or infinity makes its
@@ -409,7 +412,7 @@ int appt_scaled_product(const appt_scaled *A, const appt_blocks *W, const int32_
 /* Waits for `device` and returns APPT_ERR_DEVICE when a product on it has given up one of its
  * bounded waits since the last call of this function (its Y is then incomplete), APPT_OK
  * otherwise. For checks after the fact; a product that is given valid arguments does not wait for
- * anything outside its own kernel. */
+ * anything outside its own kernel. Not for use while a stream of the device is being captured. */
 int appt_scaled_product_status(int32_t device);
 
 const char *appt_last_error(void);

@@ -201,3 +201,20 @@ def test_operands_that_are_no_tensors():
         ex.Dispatch(routes(), D(at(0), (4, 5), "f32", (1, 4)), dense(1, 8, 5, "f32"))
     with pytest.raises(ap.ApptError, match="unknown type"):
         D(at(0), (4, 5), "e5m2")
+
+
+@pytest.mark.parametrize("op,change", [
+    ("dispatch", dict(x=dense(0, 4, 5, "bf16", ld=(1 << 31) - 2),
+                      y=D(at(1), ((1 << 31) - 2, 5), "bf16", ((1 << 31) - 2, 1)))),
+    ("combine", dict(h=D(at(1), ((1 << 31) - 2, 5), "f64", ((1 << 31) - 2, 1)))),
+    ("quantize", dict(x=D(at(1), ((1 << 31) - 2, 400), "f32", ((1 << 31) - 2, 1)),
+                      q=D(at(2), ((1 << 31) - 2, 200), "e4m3"),
+                      scale=D(at(3), (2, (1 << 31) - 2), "f32"))),
+    ("product", dict(w=D(at(2), ((1 << 30), 200), "e4m3", (1 << 36, 1)), expert_ptr=None,
+                     w_scale=D(at(3), (1 << 23, 2), "f32"),
+                     y=D(at(4), (8, 1 << 30), "bf16", (1 << 30, 1)))),
+])
+def test_operands_beyond_any_memory(op, change):
+    # the spans of these would wrap 64-bit addresses
+    message = outcome(lambda: GOOD[op](**change))
+    assert "any memory" in message, message
