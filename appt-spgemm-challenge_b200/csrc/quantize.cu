@@ -63,9 +63,11 @@ struct Values {
 };
 
 // x / s in fp32, rounded to nearest as a division is, for many x with one s: with y the rounded
-// reciprocal and q = x y, one step q + (x - q s) y corrects the last place (Markstein's method; the
-// remainder is exact in an fma). Holds while neither s, its reciprocal nor the remainder leaves the
-// normal range; other scales (and those that are no numbers) divide.
+// reciprocal and q = x y, one step q - (q s - x) y corrects the last place (Markstein's method; the
+// remainder is exact in an fma). The remainder is taken with this sign because a zero's is then a
+// zero whose product with -y has q's sign: -0 stays -0 (with x - q s it became +0). Holds while
+// neither s, its reciprocal nor the remainder leaves the normal range; other scales (and those that
+// are no numbers) divide.
 struct Divisor {
   float s, y;
   __device__ __forceinline__ explicit Divisor(float scale) {
@@ -75,7 +77,7 @@ struct Divisor {
   __device__ __forceinline__ bool holds() const { return s > 0x1p-60f && s < 0x1p60f; }
   __device__ __forceinline__ float of(float x) const {
     const float q = x * y;
-    return __fmaf_rn(__fmaf_rn(-q, s, x), y, q);
+    return __fmaf_rn(-__fmaf_rn(q, s, -x), y, q);
   }
 };
 
