@@ -321,7 +321,11 @@ class ScaledProduct(_Call):
         n, k = d.shape[-2:]
         ld = d.strides[-2] if n > 1 else -(-k // 16) * 16
         step = d.strides[0] if dims == 3 and groups > 1 else 0
-        sw = self._flat(w_scale, "w_scale", ("f32",), groups * -(-n // BLOCK) * -(-k // BLOCK), dims)
+        need = (groups, -(-n // BLOCK), -(-k // BLOCK))[3 - dims:]
+        scale = self._dense(w_scale, "w_scale", dims, ("f32",))
+        if scale.shape != need:   # blocks the other way round have as many entries
+            raise ApptError(f"w_scale: needs the shape {need}, not {scale.shape}")
+        sw = self._flat(w_scale, "w_scale", ("f32",), dims=dims)
         mw = BlocksArg(groups, n, k, ld, step, d.ptr, sw)
         ptr = self._flat(expert_ptr, "expert_ptr", ("i32",), groups + 1)
         self._set(ma, mw, ptr, self._matrix(y, "y"))

@@ -218,3 +218,24 @@ def test_operands_beyond_any_memory(op, change):
     # the spans of these would wrap 64-bit addresses
     message = outcome(lambda: GOOD[op](**change))
     assert "any memory" in message, message
+
+
+@pytest.mark.parametrize("shape", [(3, 4, 2), (2, 3, 4), (24, 1, 1), (1, 6, 4), (3, 2, 3)])
+def test_weights_scales_of_another_shape(shape):
+    """As many scales as there are blocks, or nearly, but not one for each where it belongs."""
+    long = dict(a=dense(0, 8, 400, "e4m3"), a_scale=dense(1, 4, 8, "f32"),
+                w=D(at(2), (3, 130, 400), "e4m3"))
+    message = outcome(lambda: GOOD["product"](**long, w_scale=D(at(3), shape, "f32")))
+    assert "w_scale" in message and "(3, 2, 4)" in message, message
+    one = {**long, "w": D(at(2), (130, 400), "e4m3"), "expert_ptr": None}
+    message = outcome(lambda: GOOD["product"](**one, w_scale=D(at(3), (4, 2), "f32")))
+    assert "w_scale" in message and "(2, 4)" in message, message
+
+
+@no_gpu
+def test_weights_scales_of_the_right_shape():
+    long = dict(a=dense(0, 8, 400, "e4m3"), a_scale=dense(1, 4, 8, "f32"))
+    assert NO_DEVICE in outcome(lambda: GOOD["product"](
+        **long, w=D(at(2), (3, 130, 400), "e4m3"), w_scale=D(at(3), (3, 2, 4), "f32")))
+    assert NO_DEVICE in outcome(lambda: GOOD["product"](
+        **long, w=D(at(2), (130, 400), "e4m3"), w_scale=D(at(3), (2, 4), "f32"), expert_ptr=None))
