@@ -168,6 +168,9 @@ class _Call:
     def _routes(self, r: "Routes") -> RoutesArg:
         if not isinstance(r, Routes):
             raise ApptError("routes: needs a Routes")
+        # (ctypes would cut larger numbers to the field's width)
+        if min(r.tokens, r.top_k) < 0 or max(r.tokens, r.top_k) >= 1 << 31:
+            raise ApptError("routes: needs tokens >= 0, top_k >= 1 and tokens * top_k < 2^31 - 1")
         ptr = self._flat(r.pair_row, "pair_row", ("i32",), r.tokens * r.top_k)
         return RoutesArg(r.tokens, r.top_k, 0, ptr)
 
@@ -210,7 +213,10 @@ class Routes:
 
 def route_workspace_bytes(tokens: int, top_k: int, experts: int) -> int:
     """Bytes of device workspace for Route. Calls that may run at the same time need one each."""
-    n = int(_lib().appt_route_workspace(tokens, top_k, experts))
+    n = 0
+    # (ctypes would cut larger numbers to the argument's width)
+    if 0 <= min(tokens, top_k, experts) and max(tokens, top_k, experts) < 1 << 31:
+        n = int(_lib().appt_route_workspace(tokens, top_k, experts))
     if n == 0:
         raise ApptError(f"no route of {tokens} x {top_k} pairs to {experts} experts: needs top_k "
                         f">= 1, 1 to {MAX_EXPERTS} experts and fewer than 2^31 - 1 pairs")
@@ -224,6 +230,8 @@ class Route(_Call):
 
     def __init__(self, ids, experts: int, expert_ptr, row_pair, pair_row, workspace):
         super().__init__("appt_route")
+        if not 1 <= experts <= MAX_EXPERTS:   # (ctypes would cut larger numbers)
+            raise ApptError(f"experts must lie in [1, {MAX_EXPERTS}]")
         m = self._matrix(ids, "ids", ("i32", "i64"))
         pairs = m.rows * m.cols
         if isinstance(workspace, Dense):

@@ -239,3 +239,17 @@ def test_weights_scales_of_the_right_shape():
         **long, w=D(at(2), (3, 130, 400), "e4m3"), w_scale=D(at(3), (3, 2, 4), "f32")))
     assert NO_DEVICE in outcome(lambda: GOOD["product"](
         **long, w=D(at(2), (130, 400), "e4m3"), w_scale=D(at(3), (2, 4), "f32"), expert_ptr=None))
+
+
+def test_sizes_wider_than_the_arguments():
+    """Numbers that a 32- or 64-bit argument would cut to small ones are refused as they are."""
+    for bad in ((10, 2 ** 32 + 2, 8), (2 ** 64 + 10, 2, 8), (10, 2, 2 ** 64 + 8),
+                (-2 ** 64 + 10, 2, 8), (10, -2 ** 32 + 2, 8), (10, 2, -2 ** 64 + 8)):
+        with pytest.raises(ap.ApptError, match="experts"):
+            ex.route_workspace_bytes(*bad)
+    # four tokens with 2^32 + 2 choices each, of which two would be left
+    wide = ex.Routes(4, 2 ** 32 + 2, flat(15, 4 * (2 ** 32 + 2)))
+    message = outcome(lambda: GOOD["dispatch"](routes=wide, weights=None))
+    assert "top_k" in message and NO_DEVICE not in message, message
+    message = outcome(lambda: GOOD["route"](experts=2 ** 64 + 8, expert_ptr=flat(1, 2 ** 64 + 9)))
+    assert "experts" in message and NO_DEVICE not in message, message
