@@ -290,7 +290,7 @@ class CombineGrad(_Call):
 class Quantize(_Call):
     """Rows of x to e4m3 with an f32 scale for each row and block of 128 columns: scale
     [ceil(cols / 128), rows], q [rows, cols]. gate "silu": the values are silu(x[:, :n]) * x[:, n:],
-    silu taken as 0 below -87.
+    in f32, silu taken as 0 below -87.3.
     rows_ptr (one i32 on the device): only that many rows are read and written."""
 
     def __init__(self, x, q, scale, rows_ptr=None, gate: str | None = None):

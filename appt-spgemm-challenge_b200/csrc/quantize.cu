@@ -8,15 +8,16 @@
 // round differently), at three instructions each.
 //
 // Bound by memory, but only just: some 25 (gated) instructions per element are 70 % of what the SMs
-// can issue. Gated bf16 16384 x 2048: 30 us, 5.6 TB/s (with both operands unpacked as they arrive 37,
+// can issue. Gated bf16 16384 x 2048: 31 us, 5.5 TB/s (with both operands unpacked as they arrive 37,
 // with plain divisions, exponentials and 64-bit index arithmetic 74). Routed bf16 8192 x 4096 to 8
 // experts each: 63 us, 5.5 TB/s (84 us); the scales' 4-byte writes land in rows far apart. Rows that
-// do not start on 16 bytes take twice as long: 2047 columns gated 58 us.
+// do not start on 16 bytes take twice as long: 2047 columns gated 59 us.
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <cfloat>
 #include "common.cuh"
 #include "experts.h"
+#include "tcgen05.cuh"
 #include "values.cuh"
 
 namespace appt {
@@ -81,14 +82,48 @@ struct Divisor {
   }
 };
 
-// g / (1 + exp(-g)). 2^x and the reciprocal are the hardware's (2 steps and 1); the argument's
-// rounding adds |g| 2^-24, which for g > 0 the 1 in the sum damps. Where exp(-g) passes 2^126 the
-// reciprocal is 0, as 1 / infinity is a little further on.
-__device__ __forceinline__ float silu(float g) {
-  float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.44269504f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-  return g * r;
+// v = silu(v) up, in pairs of neighbours: silu(g) = g / (1 + exp(-g)), below 10 half steps of fp32
+// with the product. 2^x and the reciprocal are the hardware's (2 steps and 1). The argument
+// -g log2(e) rounded would alone be off by |g| half steps (5e-6 at -80), so x and m have exp(-g) =
+// 2^x exp(m), m small. For 16-bit gates x is an exact product with the leading bits of log2(e) and m
+// the other bits' part; for bf16 1 + m is exp(m) but for m^2 / 2 (half a step more at -50, 1.3 at
+// -80), for fp16 the square is taken too. Else m is what rounding took from x, and exp(m) = 1 + m.
+// No branch: gates below -87.3, whose silu is smaller than 2^-119, get a reciprocal of 0 and with it
+// a 0; and an infinite gate's 0 times m is a NaN, which a maximum with 1, never above 1 + exp(-g),
+// takes away (a gate that is a NaN is a factor still). A way of its own for far gates, to where silu
+// leaves fp32 near -104, took 33 to 39 us instead of 31 even where there was none, for it cuts the
+// block's instructions in two.
+template <typename T>
+__device__ __forceinline__ void gate(float& v0, float& v1, float up0, float up1) {
+  using namespace sm100;
+  const uint64_t g = two(v0, v1);
+  uint64_t m;
+  float e0, e1;
+  if constexpr (sizeof(T) == 2) {
+    constexpr bool kHalf = std::is_same<T, __half>::value;
+    constexpr float kLog2e = kHalf ? 0x1.715p+0f : 0x1.7154p+0f;        // 13 and 15 bits
+    // the other bits, times -ln(2)
+    constexpr float kRestLn2 = kHalf ? -0x1.8be626p-15f : -0x1.480fb6p-18f;
+    untwo(mul_two(g, two(-kLog2e, -kLog2e)), e0, e1);
+    m = mul_two(g, two(kRestLn2, kRestLn2));
+    if (kHalf) m = mul_two(m, fma_two(m, two(0.5f, 0.5f), two(1.f, 1.f)));
+  } else {
+    constexpr float kLog2e = 0x1.715476p+0f, kRest = 0x1.4ae0cp-26f;   // their sum: log2(e)
+    constexpr float kLn2 = 0x1.62e43p-1f;
+    untwo(mul_two(g, two(-kLog2e, -kLog2e)), e0, e1);
+    e0 = fminf(e0, 127.f), e1 = fminf(e1, 127.f);   // no infinity times a negative m
+    m = fma_two(g, two(kLog2e, kLog2e), two(e0, e1));   // exact
+    m = fma_two(g, two(kRest, kRest), m);
+    m = mul_two(m, two(-kLn2, -kLn2));
+  }
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e0));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e1));
+  const uint64_t e = two(e0, e1);
+  untwo(add_two(fma_two(e, m, e), two(1.f, 1.f)), e0, e1);
+  e0 = fmaxf(e0, 1.f), e1 = fmaxf(e1, 1.f);
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e0));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e1));
+  untwo(mul_two(mul_two(g, two(e0, e1)), two(up0, up1)), v0, v1);
 }
 
 // max(|a|, |b|, c), a NaN where one is
@@ -163,11 +198,12 @@ __global__ void __launch_bounds__(kThreads, 5)
         float up[kPer];
         factor.unpack(up);
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) v[k] = silu(v[k]) * up[k];
+        for (int k = 0; k < kPer; k += 2) gate<T>(v[k], v[k + 1], up[k], up[k + 1]);
       }
       float top = 0.f;
 #pragma unroll
       for (int k = 0; k < kPer; k += 2) top = abs_max(v[k], v[k + 1], top);
+      
 #pragma unroll
       for (int s = L::kLanes / 2; s > 0; s >>= 1)
         top = abs_max(__shfl_xor_sync(mine, top, s), 0.f, top);

@@ -204,7 +204,7 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
       : "memory");
 }
 
-// Pairs of fp32 values in 64 bits: sum + a f, one instruction for both.
+// Pairs of fp32 values in 64 bits, one instruction for both.
 __device__ __forceinline__ uint64_t two(float lo, float hi) {
   uint64_t v;
   asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
@@ -212,6 +212,22 @@ __device__ __forceinline__ uint64_t two(float lo, float hi) {
 }
 __device__ __forceinline__ void untwo(uint64_t v, float& lo, float& hi) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t add_two(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+__device__ __forceinline__ uint64_t mul_two(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+// sum + a f
+__device__ __forceinline__ uint64_t fma_two(uint64_t a, uint64_t f, uint64_t sum) {
+  uint64_t v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(f), "l"(sum));
+  return v;
 }
 __device__ __forceinline__ uint64_t fma_two(uint32_t a0, uint32_t a1, uint64_t f, uint64_t sum) {
   uint64_t v;

@@ -388,8 +388,8 @@ int appt_combine_grad(const appt_routes *routes, const appt_dense *dY, const app
                       void *stream);
 
 #define APPT_GATE_NONE 0
-#define APPT_GATE_SILU 1 /* values are silu(X[:, :n]) * X[:, n:], n = Q's columns, X has 2 n;
-                            silu of values below -87 is 0 */
+#define APPT_GATE_SILU 1 /* values are silu(X[:, :n]) * X[:, n:] in F32, n = Q's columns, X has 2 n;
+                            silu of values below -87.3 (it is smaller than 2^-119 there) is 0 */
 
 /* Rows to 8 bits: for each row and block of 128 columns, scale = max(|largest value| / 448,
  * smallest normal float), q = value / scale rounded to nearest even. A NaN or infinity makes its

@@ -1,9 +1,10 @@
-"""Edges of the routed products' quantiser on the GPU: zeros of either sign."""
+"""Edges of the routed products' quantiser on the GPU: zeros of either sign, and gates over their
+whole range."""
 import pytest
 import torch
 
-from test_experts_gpu import (BF16, DEV, F16, F32, eight_bits, ex, gen, pair_parts, quantized, rand,
-                              routing, same_bits, stream)
+from test_experts_gpu import (BF16, DEV, F16, F32, F64, blocked, eight_bits, ex, gen, pair_parts,
+                              quantized, rand, routing, s, same_bits, stream, u)
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +65,79 @@ def test_gated_zeros_keep_their_sign(width, dtype):
     zero = (gate == 0) | (up == 0)
     assert torch.equal(negative(q)[zero], (torch.signbit(gate) ^ torch.signbit(up))[zero])
     assert (q.float()[zero] == 0).all()
+
+
+def gated(x, width):
+    gate, up = x[:, :width].double(), x[:, width:].double()
+    return gate / (1 + torch.exp(-gate)) * up
+
+
+def gated_in_fp32_range(x, width):
+    """The same where silu, and the product, are held in fp32: zero or infinite outside its range."""
+    gate, up = x[:, :width].double(), x[:, width:].double()
+    return ((gate / (1 + torch.exp(-gate))).float().double() * up).float().double()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("width", [16, 7])
+def test_gates_of_every_size(width, dtype):
+    """Gates from -104 to 104, a row of one size each, so that the row's scale shows silu itself.
+
+    Of the value in fp32: 2^x to 2 ulp, its argument's rest, the sum, the quotient to an ulp and two
+    products: below 10 half steps. bf16 takes exp(m) as 1 + m with |m| < 4.9e-6 |g|: m^2 / 2 more.
+    Below -87 silu may be 0, and where the value is subnormal it is held to half the smallest step."""
+    steps = torch.arange(-104 * 8, 104 * 8 + 1, device=DEV, dtype=F64) / 8
+    rows = steps.numel()
+    g = gen(83)
+    x = torch.empty(rows, 2 * width, device=DEV, dtype=F64)
+    x[:, :width] = steps[:, None] * rand(g, rows, width, dtype=F64, lo=0.97, hi=1.0)
+    # the factors bring the values of negative gates back to ordinary sizes
+    big = torch.exp2((-steps).clamp(0, 80).round()) if dtype != F16 else \
+        torch.exp2((-steps).clamp(0, 15).round())
+    x[:, width:] = big[:, None] * rand(g, rows, width, dtype=F64, lo=1.0, hi=1.9)
+    x = x.to(dtype)
+    q, scale = eight_bits(rows, width), torch.empty(1, rows, device=DEV)
+    ex.Quantize(x, q, scale, gate="silu").run(stream())
+    v = gated(x, width)
+    gate = x[:, :width].double()
+    part = 10 * u(F32) + ((4.9e-6 * gate) ** 2 / 2 if dtype == BF16 else 0.0)
+    off = torch.where(gate < -87, 1.0, part) * v.abs() + 1.01 * s(F32)
+    top, at = v.abs().max(1)
+    want = (top / 448).clamp(min=torch.finfo(F32).tiny)
+    worst = (scale[0].double() - want).abs() / (off.gather(1, at[:, None])[:, 0] / 448
+                                                + u(F32) * want)
+    assert worst.max() <= 1, (float(worst.max()), float(steps[worst.argmax()]))
+    step = scale[0].double()[:, None]
+    back = q.double() * step
+    bad = (back - v).abs() > 1.0001 * (v.abs() * 2 ** -4 + step * 2 ** -10) + off
+    assert not bad.any(), steps[bad.any(1)][:8]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("width", [256, 131])
+def test_gates_that_are_extreme_or_no_numbers(width, dtype):
+    """The largest and the lowest gates, infinities, NaN, and a product that overflows; each block's
+    scale and bytes as the definition has them, and no other block changed."""
+    top = torch.finfo(dtype).max
+    cases = [(top, 1.0), (-top, 1.0), (-top, -top), (float("inf"), 1.0), (float("-inf"), 1.0),
+             (float("nan"), 1.0), (1.0, float("inf")), (-200.0, float("inf")), (-200.0, top),
+             (0.0, float("inf")), (top, top), (float("-inf"), 0.0)]
+    g = gen(84)
+    x = rand(g, len(cases), 2 * width, dtype=dtype)
+    for i, (gate, up) in enumerate(cases):
+        x[i, 130], x[i, width + 130] = gate, up
+    q, scale = eight_bits(len(cases), width), torch.empty(2, len(cases), device=DEV)
+    ex.Quantize(x, q, scale, gate="silu").run(stream())
+    v = gated_in_fp32_range(x, width)
+    b = blocked(v)
+    amax = b.abs().amax(-1).t()          # keeps a NaN
+    want = (amax / 448).clamp(min=torch.finfo(F32).tiny)
+    assert torch.equal(torch.isnan(scale), torch.isnan(want))
+    assert torch.equal(torch.isinf(scale), torch.isinf(want))
+    fine = torch.isfinite(want)
+    assert ((scale - want).abs()[fine] <= 11 * u(F32) * want[fine]).all()
+    byte = q.float()[:, 130]
+    ratio = v[:, 130] / want[1]
+    assert torch.equal(torch.isnan(byte), torch.isnan(ratio))
+    assert torch.equal(negative(q)[:, 130][ratio == 0], torch.signbit(v[:, 130])[ratio == 0])
+    assert torch.isfinite(q.float()[:, :128]).all()
