@@ -42,32 +42,24 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   return done != 0;
 }
 
-// Waits are bounded: a wait of two seconds, or one that sees that another gave up, gives up. Whole
-// warps wait, and the vote keeps them together: a wait by a single thread of a warp, in a branch
-// that the others skip, measured 205 cycles on a barrier that is ready, a whole warp's 70.
-constexpr int kWaitTries = 1 << 26;
-constexpr unsigned long long kWaitNs = 2000000000ull;
-__device__ __forceinline__ unsigned long long now_ns() {
-  unsigned long long t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
+// Waits are bounded by tries, which count only while the kernel runs (a clock goes on while another
+// process has the GPU): the hardware ends a try that fails after some 4 us, so 2^19 are two seconds.
+// A wait also ends when it sees that another gave up. Whole warps wait, and the vote keeps them
+// together: a wait by a single thread of a warp, in a branch that the others skip, measured 205
+// cycles on a barrier that is ready, a whole warp's 70.
+constexpr int kWaitTries = 1 << 19;
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
-  if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
-  const unsigned long long began = now_ns();
   for (int i = 0; i < kWaitTries; ++i) {
     if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
-    if ((i & 63) == 63 &&
-        __any_sync(0xffffffffu, *gave_up != 0 || now_ns() - began > kWaitNs)) break;
+    if ((i & 63) == 63 && __any_sync(0xffffffffu, *gave_up != 0)) break;
   }
   *gave_up = 1;
   return false;
 }
 // What is still in flight when a kernel gives up, or ends: the same without the flag.
 __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
-  const unsigned long long began = now_ns();
-  for (int i = 0; i < kWaitTries && !mbar_try(bar, parity); ++i)
-    if ((i & 63) == 63 && now_ns() - began > kWaitNs) break;
+  for (int i = 0; i < kWaitTries && !mbar_try(bar, parity); ++i) {
+  }
 }
 // One thread of a converged warp; the compiler knows that it is one (a product issued under a
 // comparison of lanes took 50 cycles, under this 8).

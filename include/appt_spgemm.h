@@ -410,9 +410,11 @@ int appt_dispatch_quantize(const appt_routes *routes, const appt_dense *X, const
 int appt_scaled_product(const appt_scaled *A, const appt_blocks *W, const int32_t *group_ptr,
                         const appt_dense *Y, int32_t device, void *stream);
 /* Waits for `device` and returns APPT_ERR_DEVICE when a product on it has given up one of its
- * bounded waits since the last call of this function (its Y is then incomplete), APPT_OK
- * otherwise. For checks after the fact; a product that is given valid arguments does not wait for
- * anything outside its own kernel. Not for use while a stream of the device is being captured. */
+ * bounded waits since the last call of this function (its Y is then incomplete, although the call
+ * that queued it returned APPT_OK), APPT_OK otherwise. For checks after the fact, also after replays
+ * of a captured graph; a product that is given valid arguments does not wait for anything outside
+ * its own kernel, and only time in which the kernel runs counts (two seconds for one wait). Not for
+ * use while a stream of the device is being captured. */
 int appt_scaled_product_status(int32_t device);
 
 const char *appt_last_error(void);
