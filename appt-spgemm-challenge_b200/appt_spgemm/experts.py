@@ -79,6 +79,8 @@ def _lib() -> ct.CDLL:
     lib.appt_route_workspace.argtypes = [ct.c_int64, ct.c_int32, ct.c_int64]
     lib.appt_route_workspace.restype = ct.c_size_t
     lib.appt_scaled_product_status.argtypes, lib.appt_scaled_product_status.restype = [dev], ct.c_int
+    lib.appt_scaled_product_give_up.argtypes = [ct.c_int32]
+    lib.appt_scaled_product_give_up.restype = None
     _ready = lib
     return lib
 
@@ -343,3 +345,9 @@ def check_products(device: int = 0) -> None:
     """Waits for the device and raises if a ScaledProduct on it has given up a wait since the last
     check (its y is then incomplete)."""
     _check(_lib().appt_scaled_product_status(device), "appt_scaled_product_status")
+
+
+def make_products_give_up(on: bool) -> None:
+    """For tests of what a program does when a product gives up a wait: those that run from now on
+    do, in their first tiles."""
+    _lib().appt_scaled_product_give_up(1 if on else 0)

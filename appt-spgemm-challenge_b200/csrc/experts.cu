@@ -428,6 +428,8 @@ int appt_scaled_product(const appt_scaled* A, const appt_blocks* W, const int32_
   });
 }
 
+void appt_scaled_product_give_up(int32_t on) { scaled_product_give_up(on != 0); }
+
 int appt_scaled_product_status(int32_t device) {
   return guarded("appt_scaled_product_status", [&] {
     OnDevice on(device);

@@ -111,6 +111,8 @@ int launch_quantize(const DenseView& x, bool gated, const int* rows_ptr, const R
 // scaled_product.cu
 int launch_scaled_product(const ScaledView& a, const BlocksView& w, const int* group_ptr,
                           const DenseView& y, int sms, cudaStream_t s);
+// Makes later products give up (or not).
+void scaled_product_give_up(bool on);
 // Reads and clears the current device's record of products that gave up a wait (a cudaError_t).
 int scaled_product_status(int* gave_up);
 

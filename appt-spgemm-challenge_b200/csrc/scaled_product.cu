@@ -67,6 +67,7 @@ struct Params {
   int n_tiles;               // tiles of a row of tiles
   int step_rows, step_cols;  // from a CTA's tile to its next
   int splits_log2;           // CTAs that share a tile's K
+  bool give_up;        // asked to, after a tile's first block (before its only one)
   bool vec;            // rows of y start on 16 bytes
 };
 
@@ -332,17 +333,18 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
           if (++st == S::kStages) st = 0, phase ^= 1;
         }
       }
-      if (!ok)   // let the loads in flight land before the CTA ends
-        for (int j = max(0, it - S::kStages); j < it; ++j)
-          mbar_drain(smem_u32(&bars->full[j % S::kStages]), j / S::kStages & 1);
+      // Loads in flight land before the CTA ends: there are some where another role has given up.
+      for (int j = max(0, it - S::kStages); j < it; ++j)
+        mbar_drain(smem_u32(&bars->full[j % S::kStages]), j / S::kStages & 1);
     } else if (warp == 1) {
       // ---- products
       constexpr uint32_t idesc = instr_desc(kLanes, kCols);
       int st = 0, b = 0;
       uint32_t phase = 0, bphase = 1;
       bool ok = true;
+      const int last = p.give_up ? min(kb0 + 1, kb1 - 1) : kb1;
       for (; ok && order.more(); order.next()) {
-        for (int kb = kb0; kb < kb1; ++kb) {
+        for (int kb = kb0; kb < last; ++kb) {
           ok = mbar_wait(smem_u32(&bars->full[st]), phase, gave_up) &&
                mbar_wait(smem_u32(&bars->tempty[b]), bphase, gave_up);
           if (!ok) break;
@@ -359,6 +361,10 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
           __syncwarp();
           if (++st == S::kStages) st = 0, phase ^= 1;
           if (++b == S::kBuffers) b = 0, bphase ^= 1;
+        }
+        if (last < kb1) {
+          *gave_up = 1;
+          ok = false;
         }
       }
       // products (and their arrivals) in flight end before the CTA does
@@ -528,6 +534,7 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
       if (splits > 1 && !waited) cluster_wait();
     }
     if (!ok && lane == 0) g_product_gave_up = 1;
+    __syncwarp();
   }
   if constexpr (kSwap) {
     if (splits > 1) {
@@ -554,6 +561,8 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
     tmem_dealloc(tmem, S::kTmemColumns);
   }
 }
+
+std::atomic<bool> g_give_up{false};
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -658,6 +667,7 @@ int launch_scaled_product(const ScaledView& a, const BlocksView& w, const int* g
   p.n_blocks = (int)((w.rows + kScaleBlock - 1) / kScaleBlock);
   p.groups = (int)w.groups;
   p.type = y.type;
+  p.give_up = g_give_up.load(std::memory_order_relaxed);
   const int b = y.type == kF32 ? 4 : 2;
   p.vec = (uintptr_t)y.data % 16 == 0 && y.ld * b % 16 == 0;
   // Few rows per group: the weights as lanes, and as few columns as mostly hold a group's rows (half
@@ -684,6 +694,8 @@ int launch_scaled_product(const ScaledView& a, const BlocksView& w, const int* g
   else product<false, 256>(a, w, p, sms, s);
   return 1;
 }
+
+void scaled_product_give_up(bool on) { g_give_up.store(on, std::memory_order_relaxed); }
 
 int scaled_product_status(int* gave_up) {
   cudaError_t e = cudaMemcpyFromSymbol(gave_up, g_product_gave_up, sizeof(int));

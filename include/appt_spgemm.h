@@ -416,6 +416,10 @@ int appt_scaled_product(const appt_scaled *A, const appt_blocks *W, const int32_
  * its own kernel, and only time in which the kernel runs counts (two seconds for one wait). Not for
  * use while a stream of the device is being captured. */
 int appt_scaled_product_status(int32_t device);
+/* For tests of what a program does then: with `on` the products that the process queues (or
+ * captures) from now on give up in their first tiles, with loads and products in flight, as if a wait
+ * had run out. */
+void appt_scaled_product_give_up(int32_t on);
 
 const char *appt_last_error(void);
 int appt_device_count(void);
