@@ -79,6 +79,8 @@ def _lib() -> ct.CDLL:
     lib.appt_route_workspace.argtypes = [ct.c_int64, ct.c_int32, ct.c_int64]
     lib.appt_route_workspace.restype = ct.c_size_t
     lib.appt_scaled_product_status.argtypes, lib.appt_scaled_product_status.restype = [dev], ct.c_int
+    lib.appt_scaled_product_tile.argtypes = [ct.c_int64, ct.c_int64, ct.c_int64, ct.c_int32, vp, vp]
+    lib.appt_scaled_product_tile.restype = ct.c_int
     lib.appt_scaled_product_give_up.argtypes = [ct.c_int32]
     lib.appt_scaled_product_give_up.restype = None
     _ready = lib
@@ -339,6 +341,16 @@ class ScaledProduct(_Call):
         mw = BlocksArg(groups, n, k, ld, step, d.ptr, sw)
         ptr = self._flat(expert_ptr, "expert_ptr", ("i32",), groups + 1)
         self._set(ma, mw, ptr, self._matrix(y, "y"))
+
+
+def product_tile(rows: int, n: int, groups: int = 1, sms: int = 148) -> tuple[int, int]:
+    """Rows and columns of the tile of y that a ScaledProduct of these sizes goes by."""
+    if not 0 <= min(rows, n, groups, sms) <= max(rows, n, groups, sms) < 1 << 31:   # (cut by ctypes)
+        raise ApptError("no product has these sizes")
+    out = (ct.c_int32 * 2)()
+    _check(_lib().appt_scaled_product_tile(rows, n, groups, sms, ct.addressof(out),
+                                           ct.addressof(out) + 4), "appt_scaled_product_tile")
+    return out[0], out[1]
 
 
 def check_products(device: int = 0) -> None:

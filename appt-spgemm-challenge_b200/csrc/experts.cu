@@ -428,6 +428,18 @@ int appt_scaled_product(const appt_scaled* A, const appt_blocks* W, const int32_
   });
 }
 
+int appt_scaled_product_tile(int64_t rows, int64_t n, int64_t groups, int32_t sms,
+                             int32_t* tile_rows, int32_t* tile_cols) {
+  return guarded("appt_scaled_product_tile", [&] {
+    if (rows < 0 || rows > 1 << 30 || n < 1 || n > 1 << 30 || groups < 1 || groups > kMaxExperts ||
+        sms < 1 || sms > 1 << 16 || !tile_rows || !tile_cols)
+      refuse("no product has these sizes, or a null output");
+    const ProductTile t = scaled_product_tile(rows, n, groups, sms);
+    *tile_rows = t.rows;
+    *tile_cols = t.cols;
+  });
+}
+
 void appt_scaled_product_give_up(int32_t on) { scaled_product_give_up(on != 0); }
 
 int appt_scaled_product_status(int32_t device) {

@@ -111,6 +111,11 @@ int launch_quantize(const DenseView& x, bool gated, const int* rows_ptr, const R
 // scaled_product.cu
 int launch_scaled_product(const ScaledView& a, const BlocksView& w, const int* group_ptr,
                           const DenseView& y, int sms, cudaStream_t s);
+// The tile of Y that a product of these sizes goes by: fewer than 128 rows with the weights as lanes.
+struct ProductTile {
+  int rows, cols;
+};
+ProductTile scaled_product_tile(long long rows, long long n, long long groups, int sms);
 // Makes later products give up (or not).
 void scaled_product_give_up(bool on);
 // Reads and clears the current device's record of products that gave up a wait (a cudaError_t).

@@ -652,6 +652,30 @@ void product(const ScaledView& a, const BlocksView& w, Params p, int sms, cudaSt
 
 }  // namespace
 
+// Few rows per group: the weights as lanes, and as few columns as mostly hold a group's rows (half
+// as many again as the mean; one group's rows are known). Else the rows as lanes, unless that
+// leaves more than half of the SMs without a tile, where the other layout can split K. 256 columns
+// unless 128 fill the SMs so much better that the narrower tile's waves, four fifths as long, are
+// fewer in time. Measured, in us, as 16 | 32 | 64 columns of rows | 128 | 256 columns of weights:
+//   64 groups, 2048 x 2048:  8 rows each  50 | 50 | 53 | 58 |  53
+//                           16 rows each  54 | 50 | 54 | 61 |  56
+//                           48 rows each 120 | 79 | 57 | 63 |  57
+//                          128 rows each 276 |169 |125 | 84 |  73
+//   one group,  4096 x 4096:  48 rows      13 | 12 | 10 | 15 |  19
+//                            512 rows      68 | 44 | 29 | 17 |  21
+//                           1024 rows     130 | 73 | 52 | 29 |  22
+//   one group,  512 x 2048:  128 rows       9 |  7 |  7 | 10 |  13
+ProductTile scaled_product_tile(long long rows, long long n, long long groups, int sms) {
+  const long long fits = groups == 1 ? rows : rows * 3 / 2 / groups;
+  const long long row_tiles = row_tiles_for(rows, groups, kLanes);
+  const long long narrow = row_tiles * ((n + 127) / 128), wide = row_tiles * ((n + 255) / 256);
+  auto waves = [&](long long tiles) { return (tiles + sms - 1) / sms; };
+  if (fits <= 16) return {16, kLanes};
+  if (fits <= 32) return {32, kLanes};
+  if (fits <= 64 || narrow * 2 <= sms) return {64, kLanes};
+  return {kLanes, waves(wide) * 5 > waves(narrow) * 4 ? 128 : 256};
+}
+
 int launch_scaled_product(const ScaledView& a, const BlocksView& w, const int* group_ptr,
                           const DenseView& y, int sms, cudaStream_t s) {
   Params p;
@@ -670,27 +694,11 @@ int launch_scaled_product(const ScaledView& a, const BlocksView& w, const int* g
   p.give_up = g_give_up.load(std::memory_order_relaxed);
   const int b = y.type == kF32 ? 4 : 2;
   p.vec = (uintptr_t)y.data % 16 == 0 && y.ld * b % 16 == 0;
-  // Few rows per group: the weights as lanes, and as few columns as mostly hold a group's rows (half
-  // as many again as the mean; one group's rows are known). Else the rows as lanes, unless that
-  // leaves more than half of the SMs without a tile, where the other layout can split K. 256 columns
-  // unless 128 fill the SMs so much better that the narrower tile's waves, four fifths as long, are
-  // fewer in time. Measured, in us, as 16 | 32 | 64 columns of rows | 128 | 256 columns of weights:
-  //   64 groups, 2048 x 2048:  8 rows each  50 | 50 | 53 | 58 |  53
-  //                           16 rows each  54 | 50 | 54 | 61 |  56
-  //                           48 rows each 120 | 79 | 57 | 63 |  57
-  //                          128 rows each 276 |169 |125 | 84 |  73
-  //   one group,  4096 x 4096:  48 rows      13 | 12 | 10 | 15 |  19
-  //                            512 rows      68 | 44 | 29 | 17 |  21
-  //                           1024 rows     130 | 73 | 52 | 29 |  22
-  //   one group,  512 x 2048:  128 rows       9 |  7 |  7 | 10 |  13
-  const long long fits = p.groups == 1 ? p.rows : p.rows * 3ll / 2 / p.groups;
-  const long long row_tiles = row_tiles_for(p.rows, p.groups, kLanes);
-  const long long narrow = row_tiles * ((p.n + 127) / 128), wide = row_tiles * ((p.n + 255) / 256);
-  auto waves = [&](long long tiles) { return (tiles + sms - 1) / sms; };
-  if (fits <= 16) product<true, 16>(a, w, p, sms, s);
-  else if (fits <= 32) product<true, 32>(a, w, p, sms, s);
-  else if (fits <= 64 || narrow * 2 <= sms) product<true, 64>(a, w, p, sms, s);
-  else if (waves(wide) * 5 > waves(narrow) * 4) product<false, 128>(a, w, p, sms, s);
+  const ProductTile tile = scaled_product_tile(p.rows, p.n, p.groups, sms);
+  if (tile.rows == 16) product<true, 16>(a, w, p, sms, s);
+  else if (tile.rows == 32) product<true, 32>(a, w, p, sms, s);
+  else if (tile.rows == 64) product<true, 64>(a, w, p, sms, s);
+  else if (tile.cols == 128) product<false, 128>(a, w, p, sms, s);
   else product<false, 256>(a, w, p, sms, s);
   return 1;
 }

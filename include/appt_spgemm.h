@@ -409,6 +409,11 @@ int appt_dispatch_quantize(const appt_routes *routes, const appt_dense *X, const
  * F32 and must not overflow there. */
 int appt_scaled_product(const appt_scaled *A, const appt_blocks *W, const int32_t *group_ptr,
                         const appt_dense *Y, int32_t device, void *stream);
+/* The tile of Y, tile_rows x tile_cols, by which appt_scaled_product computes a Y of rows x n in
+ * `groups` groups on a GPU of `sms` SMs (host only; for tests and for reading measurements): 16, 32
+ * or 64 rows x 128 with the weights as the tensor cores' lanes, 128 rows x 128 or 256 otherwise. */
+int appt_scaled_product_tile(int64_t rows, int64_t n, int64_t groups, int32_t sms,
+                             int32_t *tile_rows, int32_t *tile_cols);
 /* Waits for `device` and returns APPT_ERR_DEVICE when a product on it has given up one of its
  * bounded waits since the last call of this function (its Y is then incomplete, although the call
  * that queued it returned APPT_OK), APPT_OK otherwise. For checks after the fact, also after replays

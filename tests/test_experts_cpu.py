@@ -253,3 +253,19 @@ def test_sizes_wider_than_the_arguments():
     assert "top_k" in message and NO_DEVICE not in message, message
     message = outcome(lambda: GOOD["route"](experts=2 ** 64 + 8, expert_ptr=flat(1, 2 ** 64 + 9)))
     assert "experts" in message and NO_DEVICE not in message, message
+
+
+@pytest.mark.parametrize("rows,n,groups,tile", [
+    (1, 4096, 1, (16, 128)), (16, 4096, 1, (16, 128)), (17, 4096, 1, (32, 128)),
+    (128, 4096, 64, (16, 128)), (64, 8192, 1, (64, 128)), (513, 640, 1, (64, 128)),
+    (1300, 1000, 1, (128, 128)), (2500, 1000, 1, (128, 256)), (32768, 2048, 64, (128, 256)),
+    (8192, 8192, 1, (128, 256)), (0, 64, 1, (16, 128)), (1 << 30, 1 << 30, 1024, (128, 256))])
+def test_tile_of_a_product(rows, n, groups, tile):
+    assert ex.product_tile(rows, n, groups) == tile
+
+
+def test_tile_of_no_product():
+    for bad in ((-1, 64, 1), (4, 0, 1), (4, 64, 0), (4, 64, 1025), (2 ** 32 + 4, 64, 1),
+                (4, 64, 1, 0), (4, 2 ** 64 + 64, 1)):
+        with pytest.raises(ap.ApptError, match="sizes"):
+            ex.product_tile(*bad)
