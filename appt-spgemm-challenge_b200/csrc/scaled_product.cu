@@ -147,7 +147,8 @@ __device__ __noinline__ void store_boxes(T* y, long long ldy, bool vec, const ch
 // copies while the warp goes on with its next tile. The 16-byte pieces of a row change places by
 // the row (the 128-byte swizzle), which spreads the threads over the banks. Stores from registers
 // are 16 bytes of 32 rows at a time and took 4,500 cycles a tile, this takes a quarter.
-// A group's last rows, and rows that TMA cannot address, are stored from the boxes instead.
+// A group's last rows, rows that TMA cannot address, and columns of which the last 16 bytes are not
+// all Y's (TMA would write the whole piece) are stored from the boxes instead.
 template <typename T, int N, int kBoxes>
 __device__ __forceinline__ void write_rows(const Params& p, const CUtensorMap* map, char* boxes,
                                            const uint64_t* v, int row, int rows, int n) {
@@ -167,7 +168,7 @@ __device__ __forceinline__ void write_rows(const Params& p, const CUtensorMap* m
       o.down(f);
       *(Pack<T, kPer>*)(box + lane * 128 + ((c % kCols) / kPer ^ (lane & 7)) * 16) = o;
     }
-    if (p.vec && rows >= 32) {
+    if (p.vec && rows >= 32 && (p.n % kPer == 0 || n + c0 + kBoxes * kCols <= p.n)) {
       bulk_fence();
       __syncwarp();
       if (lane == 0) {
