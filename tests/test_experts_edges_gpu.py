@@ -1,10 +1,10 @@
-"""Edges of the routed products' quantiser on the GPU: zeros of either sign, and gates over their
-whole range."""
+"""Edges of the routed products on the GPU: the quantiser's zeros of either sign, gates over their
+whole range, and far rows."""
 import pytest
 import torch
 
-from test_experts_gpu import (BF16, DEV, F16, F32, F64, blocked, eight_bits, ex, gen, pair_parts,
-                              quantized, rand, routing, s, same_bits, stream, u)
+from test_experts_gpu import (BF16, DEV, E4M3, F16, F32, F64, blocked, eight_bits, ex, gen,
+                              pair_parts, quantized, rand, routing, s, same_bits, stream, u)
 
 pytestmark = pytest.mark.gpu
 
@@ -141,3 +141,40 @@ def test_gates_that_are_extreme_or_no_numbers(width, dtype):
     assert torch.equal(torch.isnan(byte), torch.isnan(ratio))
     assert torch.equal(negative(q)[:, 130][ratio == 0], torch.signbit(v[:, 130])[ratio == 0])
     assert torch.isfinite(q.float()[:, :128]).all()
+
+
+def test_far_rows():
+    """Rows past 2^32 bytes in the gradients and in both quantisers, plain and gated."""
+    k, rows = 1 << 16, (1 << 16) + 40
+    g = gen(85)
+    at = torch.tensor([rows - 1, 0, rows - 2], device=DEV)
+    r = ex.Routes(3, 1, at.to(torch.int32))
+    w = rand(g, 3, 1)
+    dy, some = rand(g, 3, k, dtype=BF16), rand(g, 3, k, dtype=BF16)
+    h = torch.zeros(rows, k, dtype=BF16, device=DEV)
+    h[at] = some
+    dh = torch.zeros(rows, k, dtype=BF16, device=DEV)
+    dw = torch.empty(3, 1, device=DEV)
+    ex.CombineGrad(r, dy, h, weights=w, dh=dh, dweights=dw).run(stream())
+    want = dy.double() * w.double()
+    assert ((dh[at].double() - want).abs() <= (u(BF16) + u(F32)) * 1.01 * want.abs()).all()
+    term = dy.double() * some.double()
+    assert ((dw[:, 0].double() - term.sum(1)).abs() <= k * u(F32) * term.abs().sum(1)).all()
+    assert not dh[1:rows - 2].any()
+    del dh
+    # plain, and as a gate of half the columns
+    q = torch.zeros(rows, k, dtype=torch.uint8, device=DEV).view(E4M3)
+    scale = torch.empty(k // 128, rows, device=DEV)
+    ex.Quantize(h, q, scale).run(stream())
+    want_q, want_scale = quantized(some)
+    assert same_bits(q[at], want_q) and torch.equal(scale[:, at], want_scale)
+    half = k // 2
+    ex.Quantize(h, q[:, :half], scale[:half // 128], gate="silu").run(stream())
+    v = gated(some, half)
+    step = scale[:half // 128, at].t().double().repeat_interleave(128, 1)
+    back = q[at, :half].double() * step
+    assert ((back - v).abs() <= 1.0001 * (v.abs() * 2 ** -4 + step * 2 ** -10)).all()
+    q.view(torch.uint8).zero_()
+    ex.DispatchQuantize(r, some, q, scale).run(stream())
+    assert same_bits(q[at], want_q) and torch.equal(scale[:, at], want_scale)
+    assert not q[1:rows - 2].view(torch.uint8).any()
