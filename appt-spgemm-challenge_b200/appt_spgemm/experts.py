@@ -355,7 +355,7 @@ def product_tile(rows: int, n: int, groups: int = 1, sms: int = 148) -> tuple[in
 
 def check_products(device: int = 0) -> None:
     """Waits for the device and raises if a ScaledProduct on it has given up a wait since the last
-    check (its y is then incomplete)."""
+    check (its y then holds NaN where it was not computed)."""
     _check(_lib().appt_scaled_product_status(device), "appt_scaled_product_status")
 
 

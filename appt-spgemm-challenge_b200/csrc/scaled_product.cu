@@ -420,6 +420,11 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
 #pragma unroll
       for (int c = 0; c < kPart / 2; ++c) pairs[c] = 0;
     };
+    // What a warp that gave up has not computed leaves as NaN, this tile and the CTA's next ones.
+    auto incomplete = [&] {
+#pragma unroll
+      for (int c = 0; c < kPart / 2; ++c) pairs[c] = ~0ull;
+    };
     if constexpr (!kSwap) {
       // A thread's scales come two blocks ahead, those of its next tile before it writes this one.
       const float *pa, *pw;
@@ -466,7 +471,7 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
           block(a0, w0, kb);
           if (ok && kb + 1 < p.k_blocks) block(a1, w1, kb + 1);
         }
-        if (!ok) break;
+        if (!ok) incomplete();
         const Tile done = t;
         order.next();
         if (order.more()) begin(t = order.at());
@@ -486,7 +491,7 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
       for (; order.more(); order.next()) {
         const Tile t = order.at();
         clear();
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        for (int kb = kb0; ok && kb < kb1; ++kb, ++it) {
           const int st = it % kScaleStages;
           ok = mbar_wait(smem_u32(&bars->sfull[st]), it / kScaleStages & 1, gave_up);
           if (!ok) break;
@@ -507,7 +512,7 @@ __global__ void __launch_bounds__(Shape<kSwap, kCols>::kThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&bars->sempty[st]));
         }
-        if (!ok) break;
+        if (!ok) incomplete();
         float sum[kPart];
 #pragma unroll
         for (int c = 0; c < kPart; c += 2) untwo(pairs[c / 2], sum[c], sum[c + 1]);

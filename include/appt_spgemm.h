@@ -415,8 +415,8 @@ int appt_scaled_product(const appt_scaled *A, const appt_blocks *W, const int32_
 int appt_scaled_product_tile(int64_t rows, int64_t n, int64_t groups, int32_t sms,
                              int32_t *tile_rows, int32_t *tile_cols);
 /* Waits for `device` and returns APPT_ERR_DEVICE when a product on it has given up one of its
- * bounded waits since the last call of this function (its Y is then incomplete, although the call
- * that queued it returned APPT_OK), APPT_OK otherwise. For checks after the fact, also after replays
+ * bounded waits since the last call of this function (its Y then holds NaN where it has not been
+ * computed, although the call that queued it returned APPT_OK), APPT_OK otherwise. For checks after the fact, also after replays
  * of a captured graph; a product that is given valid arguments does not wait for anything outside
  * its own kernel, and only time in which the kernel runs counts (two seconds for one wait). Not for
  * use while a stream of the device is being captured. */

@@ -26,8 +26,8 @@ def giving_up():
 
 @pytest.mark.parametrize("rows,n,k,groups", GIVING_UP)
 def test_a_product_that_gives_up(rows, n, k, groups, giving_up):
-    """It ends, writes nothing outside its rows and columns, and is reported once; the next one on
-    the same buffers is right."""
+    """It ends, leaves NaN where it has not computed, which here is everywhere, and nothing outside
+    its rows and columns, and is reported once; the next one on the same buffers is right."""
     g = gen(90)
     a, sa = activations(g, rows, k)
     w, sw = weights(g, groups, n, k)
@@ -39,6 +39,7 @@ def test_a_product_that_gives_up(rows, n, k, groups, giving_up):
     with pytest.raises(ap.ApptError, match="gave up"):
         ex.check_products()
     ex.check_products()
+    assert torch.isnan(base[1:rows + 1, :n]).all()
     for outside in (base[0], base[rows + 1:], base[:, n:]):
         assert (outside == 9.0).all()
     ex.make_products_give_up(False)
@@ -48,6 +49,28 @@ def test_a_product_that_gives_up(rows, n, k, groups, giving_up):
     close(base[1:rows + 1, :n], want, product_tol(want, size, k, F32))
     for outside in (base[0], base[rows + 1:], base[:, n:]):
         assert (outside == 9.0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,n", [(3, 260), (60, 260), (1300, 1037), (2500, 1037)])
+def test_what_reads_a_product_that_gave_up(rows, n, dtype, giving_up):
+    """The next steps of a layer get NaN, not the buffer's old values: rows of no group keep theirs."""
+    g = gen(98)
+    k = 700
+    a, sa = activations(g, rows, k)
+    w, sw = weights(g, 2, n, k)
+    y = torch.full((rows, n + n % 2), 9.0, device=DEV, dtype=dtype)
+    ptr = [1, rows // 2, rows - 1]
+    dptr = torch.tensor(ptr, dtype=torch.int32, device=DEV)
+    q = torch.zeros(rows, n // 2, dtype=torch.uint8, device=DEV).view(E4M3)
+    scale = torch.zeros(-(-(n // 2) // 128), rows, device=DEV)
+    ex.ScaledProduct(a, sa, w, sw, y[:, :n], expert_ptr=dptr).run(stream())
+    ex.Quantize(y[:, :n // 2 * 2], q, scale, gate="silu").run(stream())
+    with pytest.raises(ap.ApptError, match="gave up"):
+        ex.check_products()
+    assert torch.isnan(y[1:rows - 1, :n]).all() and torch.isnan(scale[:, 1:rows - 1]).all()
+    assert (y[0] == 9.0).all() and (y[rows - 1] == 9.0).all() and (y[:, n:] == 9.0).all()
+    assert torch.isfinite(scale[:, 0]).all()
 
 
 def test_a_captured_product_that_gives_up(giving_up):
