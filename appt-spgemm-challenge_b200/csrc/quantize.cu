@@ -203,7 +203,6 @@ __global__ void __launch_bounds__(kThreads, 5)
       float top = 0.f;
 #pragma unroll
       for (int k = 0; k < kPer; k += 2) top = abs_max(v[k], v[k + 1], top);
-      
 #pragma unroll
       for (int s = L::kLanes / 2; s > 0; s >>= 1)
         top = abs_max(__shfl_xor_sync(mine, top, s), 0.f, top);

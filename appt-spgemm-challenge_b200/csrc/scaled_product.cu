@@ -23,11 +23,11 @@
 // the ranks, so the result does not depend on timing.
 //
 // Many rows: no unit is full (tensor pipe 55 %, issue slots 44 %, DRAM 8 %); the adding warps' chain
-// sets the time. A block of 128 x 256 takes the tensor cores 512 cycles and the adding warps some 820:
-// 256 for its fused multiply-adds, about as much for the reads of tensor memory between them, which do
-// not overlap, the rest for waiting on one buffer and handing back the other. Neither more adding warps (4 warpgroups of 64 columns), nor pairs of CTAs on tiles of 256
-// rows (a third less traffic from L2), nor halves of 128 columns with barriers of their own were
-// faster. 8192 x 8192 x 4096 takes 259 us, 2.1 PFLOP/s (300 us at the clocks that 1000 W leave it),
+// sets the time. A block of 128 x 256 takes the tensor cores 512 cycles and the adding warps some
+// 820: 256 for its fused multiply-adds, about as much for the reads of tensor memory between them,
+// which do not overlap, the rest for waiting on one buffer and handing back the other. Neither more
+// adding warps (4 warpgroups of 64 columns), nor pairs of CTAs on tiles of 256 rows (a third less
+// traffic from L2), nor halves of 128 columns with barriers of their own were faster. 8192 x 8192 x 4096 takes 259 us, 2.1 PFLOP/s (300 us at the clocks that 1000 W leave it),
 // 32,768 sorted rows x 2048 x 2048 over 64 groups 174 us. Few rows: bound by the weights' bytes;
 // 128 rows over 56 of 64 groups, 4096 x 2048, 78 us, 6.1 TB/s; one row x 4096 x 4096 6.2 us.
 #include <cuda.h>

@@ -416,10 +416,10 @@ int appt_scaled_product_tile(int64_t rows, int64_t n, int64_t groups, int32_t sm
                              int32_t *tile_rows, int32_t *tile_cols);
 /* Waits for `device` and returns APPT_ERR_DEVICE when a product on it has given up one of its
  * bounded waits since the last call of this function (its Y then holds NaN where it has not been
- * computed, although the call that queued it returned APPT_OK), APPT_OK otherwise. For checks after the fact, also after replays
- * of a captured graph; a product that is given valid arguments does not wait for anything outside
- * its own kernel, and only time in which the kernel runs counts (two seconds for one wait). Not for
- * use while a stream of the device is being captured. */
+ * computed, although the call that queued it returned APPT_OK), APPT_OK otherwise. For checks after
+ * the fact, also after replays of a captured graph; a product that is given valid arguments does not
+ * wait for anything outside its own kernel, and only time in which the kernel runs counts (two
+ * seconds for one wait). Not for use while a stream of the device is being captured. */
 int appt_scaled_product_status(int32_t device);
 /* For tests of what a program does then: with `on` the products that the process queues (or
  * captures) from now on give up in their first tiles, with loads and products in flight, as if a wait
