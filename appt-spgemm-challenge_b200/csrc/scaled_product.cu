@@ -27,9 +27,10 @@
 // 820: 256 for its fused multiply-adds, about as much for the reads of tensor memory between them,
 // which do not overlap, the rest for waiting on one buffer and handing back the other. Neither more
 // adding warps (4 warpgroups of 64 columns), nor pairs of CTAs on tiles of 256 rows (a third less
-// traffic from L2), nor halves of 128 columns with barriers of their own were faster. 8192 x 8192 x 4096 takes 259 us, 2.1 PFLOP/s (300 us at the clocks that 1000 W leave it),
-// 32,768 sorted rows x 2048 x 2048 over 64 groups 174 us. Few rows: bound by the weights' bytes;
-// 128 rows over 56 of 64 groups, 4096 x 2048, 78 us, 6.1 TB/s; one row x 4096 x 4096 6.2 us.
+// traffic from L2), nor halves of 128 columns with barriers of their own were faster. 8192 x 8192 x
+// 4096 takes 259 us, 2.1 PFLOP/s (300 us at the clocks that 1000 W leave it), 32,768 sorted rows x
+// 2048 x 2048 over 64 groups 174 us. Few rows: bound by the weights' bytes; 128 rows over 56 of 64
+// groups, 4096 x 2048, 78 us, 6.1 TB/s; one row x 4096 x 4096 6.2 us.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <climits>
